@@ -33,8 +33,12 @@ COMMON = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-I", os.path.
 # faster than under the iterative ILP strategy at the fp16 and fp32 bench shapes).  The fp16
 # forward (three waves per SIMD in 168 VGPRs) gains 4-6% at 2-4 heads x 12 batches of 2048 under
 # the iterative ILP strategy; the fp32 forward runs best under the default one.
+# The cache and draft kernels meet stored NaN and invalid probabilities and test for them, so these two files
+# keep IEEE comparisons.
+_IEEE = ["-fhonor-nans", "-mamdgpu-ieee"]
 _BWD = ["-mllvm", "-amdgpu-sched-strategy=iterative-maxocc"]
 PER_FILE = {"fpa_bwd_fused.hip": _BWD, "fpa_bwd_kv.hip": _BWD, "fpa_bwd_q.hip": _BWD,
+            "fpa_cache.hip": _IEEE, "fpa_verify.hip": _IEEE,
             "fpa_fwd16.hip": ["-mllvm", "-amdgpu-sched-strategy=iterative-ilp"]}
 
 

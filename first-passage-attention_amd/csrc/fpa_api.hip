@@ -11,6 +11,7 @@
 #include "fpa.h"
 #include "fpa_common.h"
 #include "fpa_params.h"
+#include "fpa_serve.h"
 
 using namespace fpa;
 
@@ -150,7 +151,7 @@ FwdWs fwd_ws(int64_t B, int64_t H, int64_t T, int64_t D, int32_t dtype) {
 
 extern "C" {
 
-int fpa_abi_version(void) { return 5; }
+int fpa_abi_version(void) { return 6; }
 
 const char *fpa_source_hash(void) { return FPA_SOURCE_HASH; }
 
@@ -393,6 +394,166 @@ int fpa_bwd_noalloc(const FpaBwdArgs *a, void *stream) {
     void *ws = scratch_of_current_device();
     if (ws == nullptr) return FPA_ERR_HIP;
     return bwd_impl(a, ws, stream, split_ok);
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------------------
+// Serving
+// ---------------------------------------------------------------------------
+namespace {
+
+int check_pages(const FpaPages &c) {
+    if (c.pages < 1 || c.H < 1) return fail(FPA_ERR_INVALID, "a cache has at least one page and one head");
+    if (c.D < 16 || (c.D & (c.D - 1)) != 0) return fail(FPA_ERR_INVALID, "the head dimension must be a power of two >= 16");
+    if (!supported_d(0, (int)(c.D > 1024 ? 1024 : c.D)))
+        return fail(FPA_ERR_UNSUPPORTED, "head dimension " + std::to_string(c.D) + " is not built (16, 32, 64, 128, 256)");
+    if (c.store != FPA_F16 && c.store != FPA_F32 && c.store != FPA_E4M3)
+        return fail(FPA_ERR_INVALID, "a cache holds fp16, fp32 or e4m3");
+    if (c.pages >= (int64_t(1) << 31) || c.H > 65535)
+        return fail(FPA_ERR_UNSUPPORTED, "a cache has fewer than 2^31 pages and at most 65535 heads");
+    const void *all[] = {c.k, c.v, c.phi, c.psi, c.phi_min, c.k_exp, c.v_exp};
+    for (int i = 0; i < (c.store == FPA_E4M3 ? 7 : 5); ++i) {
+        if (!all[i]) return fail(FPA_ERR_INVALID, "a buffer of the cache is NULL");
+        if ((reinterpret_cast<uintptr_t>(all[i]) & 15) != 0) return fail(FPA_ERR_INVALID, "the cache's buffers must be 16-byte aligned");
+    }
+    return FPA_OK;
+}
+
+// What the calls on a cache have in common.
+int check_serve(const FpaPages &c, int64_t B, int64_t N, int64_t P, int32_t dtype, const void *table, const void *at) {
+    if (int rc = check_pages(c)) return rc;
+    if (B < 1 || N < 1 || P < 1) return fail(FPA_ERR_INVALID, "B, N and the table's width must be at least 1");
+    if (dtype != FPA_F16 && dtype != FPA_F32) return fail(FPA_ERR_INVALID, "the tensors must be fp16 or fp32");
+    if (c.store != FPA_E4M3 && dtype != c.store) return fail(FPA_ERR_INVALID, "the tensors must have the cache's type");
+    if (B > 65535) return fail(FPA_ERR_UNSUPPORTED, "B must be at most 65535");
+    if (N > MAX_NB * G || P > MAX_NB) return fail(FPA_ERR_UNSUPPORTED, "at most " + std::to_string(MAX_NB) + " pages (8388608 positions) a sequence");
+    if (!table || !at) return fail(FPA_ERR_INVALID, "the table and the lengths must be non-NULL");
+    return FPA_OK;
+}
+
+Pages pages_of(const FpaPages &c) {
+    Pages g;
+    g.k = c.k; g.v = c.v;
+    g.phi = c.phi; g.psi = c.psi; g.phi_min = c.phi_min;
+    g.k_exp = c.k_exp; g.v_exp = c.v_exp;
+    g.n = c.pages; g.H = (int)c.H;
+    return g;
+}
+
+// Parts of the sequences' own pages and of the prefix, and their scratch.
+struct AttendPlan {
+    int chunk, nchunk, pchunk = 1, npchunk = 0;
+    int64_t ml, total;  // float offset of the statistics, bytes
+};
+AttendPlan attend_plan(int64_t B, int64_t H, int64_t N, int64_t D, int64_t P, int64_t PL) {
+    AttendPlan a;
+    attend_parts(B * H * ((N + 15) / 16), P, a.chunk, a.nchunk);
+    if (PL > 0) attend_parts(H * ((B * N + 15) / 16), (PL + PG - 1) / PG, a.pchunk, a.npchunk);
+    const int64_t slots = (a.nchunk <= 1 && a.npchunk == 0) ? 0 : (int64_t)(a.nchunk + a.npchunk) * B * H * N;
+    a.ml = align64(slots * D);
+    a.total = (a.ml + align64(slots * 2)) * (int64_t)sizeof(float);
+    return a;
+}
+
+}  // namespace
+
+extern "C" {
+
+int fpa_cache_append(const FpaAppendArgs *a, void *stream) {
+    g_err.clear();
+    if (a == nullptr) return fail(FPA_ERR_INVALID, "args is NULL");
+    int rc = check_serve(a->cache, a->B, a->N, a->P, a->dtype, a->table, a->start);
+    if (rc) return rc;
+    if ((rc = check_rows(a->k, a->sk, a->dtype, "k")) || (rc = check_rows(a->v, a->sv, a->dtype, "v"))) return rc;
+    if (a->sk[3] != 1 || a->sv[3] != 1) return fail(FPA_ERR_INVALID, "the head dimension of k and v must be contiguous");
+    if (!a->phi || !a->psi) return fail(FPA_ERR_INVALID, "phi and psi must be non-NULL");
+    MoveParams p = {};
+    p.c = pages_of(a->cache);
+    p.k = a->k; p.sk = s3(a->sk);
+    p.v = a->v; p.sv = s3(a->sv);
+    p.phi = a->phi; p.sphi = s3(a->sphi);
+    p.psi = a->psi; p.spsi = s3(a->spsi);
+    p.table = a->table; p.stable = a->stable; p.start = a->start; p.counts = a->counts;
+    p.B = (int)a->B; p.N = (int)a->N; p.P = (int)a->P; p.D = (int)a->cache.D;
+    const hipError_t e = launch_append(p, a->dtype, a->cache.store, reinterpret_cast<hipStream_t>(stream));
+    return e != hipSuccess ? hip_fail(e, "fpa_cache_append launch") : FPA_OK;
+}
+
+int fpa_cache_read(const FpaReadArgs *a, void *stream) {
+    g_err.clear();
+    if (a == nullptr) return fail(FPA_ERR_INVALID, "args is NULL");
+    int rc = check_serve(a->cache, a->B, a->N, a->P, a->dtype, a->table, a->start);
+    if (rc) return rc;
+    if (!a->k || !a->v || !a->phi || !a->psi) return fail(FPA_ERR_INVALID, "k, v, phi and psi must be non-NULL");
+    if (((reinterpret_cast<uintptr_t>(a->k) | reinterpret_cast<uintptr_t>(a->v)) & 15) != 0)
+        return fail(FPA_ERR_INVALID, "k and v must be 16-byte aligned");
+    MoveParams p = {};
+    p.c = pages_of(a->cache);
+    p.ko = a->k; p.vo = a->v; p.phio = a->phi; p.psio = a->psi;
+    p.table = a->table; p.stable = a->stable; p.start = a->start; p.counts = a->counts;
+    p.B = (int)a->B; p.N = (int)a->N; p.P = (int)a->P; p.D = (int)a->cache.D;
+    const hipError_t e = launch_read(p, a->dtype, a->cache.store, reinterpret_cast<hipStream_t>(stream));
+    return e != hipSuccess ? hip_fail(e, "fpa_cache_read launch") : FPA_OK;
+}
+
+int64_t fpa_attend_workspace_bytes(int64_t B, int64_t H, int64_t N, int64_t D, int64_t P, int64_t prefix_length) {
+    if (B < 1 || H < 1 || N < 1 || D < 1 || P < 1) return 0;
+    return attend_plan(B, H, N, D, P, prefix_length).total;
+}
+
+int fpa_attend(const FpaAttendArgs *a, void *stream) {
+    g_err.clear();
+    if (a == nullptr) return fail(FPA_ERR_INVALID, "args is NULL");
+    int rc = check_serve(a->cache, a->B, a->N, a->P, a->dtype, a->table, a->lengths);
+    if (rc) return rc;
+    if ((rc = check_rows(a->q, a->sq, a->dtype, "q"))) return rc;
+    if (a->sq[3] != 1 || a->so[3] != 1) return fail(FPA_ERR_INVALID, "the head dimension of q and o must be contiguous");
+    if (!a->o || !a->beta) return fail(FPA_ERR_INVALID, "o and beta must be non-NULL");
+    if (a->prefix_length < 0 || a->prefix_length > (int64_t)MAX_NB * G)
+        return fail(FPA_ERR_INVALID, "prefix_length must be between 0 and " + std::to_string((int64_t)MAX_NB * G));
+    if (a->prefix_length > 0 && !a->prefix) return fail(FPA_ERR_INVALID, "prefix is NULL");
+    const int64_t H = a->cache.H, D = a->cache.D;
+    const AttendPlan pl = attend_plan(a->B, H, a->N, D, a->P, a->prefix_length);
+    if (pl.total > 0 && (a->workspace == nullptr || (reinterpret_cast<uintptr_t>(a->workspace) & 255) != 0))
+        return fail(FPA_ERR_INVALID, "workspace must be non-NULL and 256-byte aligned");
+    // One workgroup per part and row tile, one merge thread per output element: grids below 2^31.
+    if ((double)a->B * H * a->N * (pl.nchunk + pl.npchunk) >= 2147483648.0 || (double)a->B * H * a->N * D / 256 >= 2147483647.0)
+        return fail(FPA_ERR_UNSUPPORTED, "B * H * N is too large");
+    AttendParams p = {};
+    p.c = pages_of(a->cache);
+    p.q = a->q; p.sq = s3(a->sq);
+    p.o = a->o; p.so = s3(a->so);
+    p.beta = a->beta;
+    p.table = a->table; p.stable = a->stable; p.lengths = a->lengths; p.prefix = a->prefix;
+    p.part = static_cast<float *>(a->workspace);
+    p.ml = p.part + pl.ml;
+    p.B = (int)a->B; p.N = (int)a->N; p.P = (int)a->P; p.PL = (int)a->prefix_length;
+    p.chunk = pl.chunk; p.nchunk = pl.nchunk; p.pchunk = pl.pchunk; p.npchunk = pl.npchunk;
+    p.sc2 = LOG2E / sqrtf((float)D);
+    const hipError_t e = launch_attend(p, a->dtype, a->cache.store, (int)D, reinterpret_cast<hipStream_t>(stream));
+    return e != hipSuccess ? hip_fail(e, "fpa_attend launch") : FPA_OK;
+}
+
+int fpa_verify(const FpaVerifyArgs *a, void *stream) {
+    g_err.clear();
+    if (a == nullptr) return fail(FPA_ERR_INVALID, "args is NULL");
+    if (a->B < 1 || a->N < 0 || a->V < 1) return fail(FPA_ERR_INVALID, "target must be (B, N + 1, V) with B, V >= 1");
+    if (a->dtype != FPA_F16 && a->dtype != FPA_F32) return fail(FPA_ERR_INVALID, "the probabilities must be fp16 or fp32");
+    if (a->B > 65535 || a->N > (1 << 20) || a->V > (1 << 30))
+        return fail(FPA_ERR_UNSUPPORTED, "B must be at most 65535, N at most 2^20 and V at most 2^30");
+    if (!a->target || !a->sample_u || !a->accepted || !a->out || (a->N > 0 && (!a->tokens || !a->accept_u)))
+        return fail(FPA_ERR_INVALID, "target, tokens, accept_u, sample_u, accepted and out must be non-NULL");
+    VerifyParams p = {};
+    p.target = a->target; p.stb = a->st[0]; p.stn = a->st[1];
+    p.draft = a->N > 0 ? a->draft : nullptr; p.sdb = a->sd[0]; p.sdn = a->sd[1];
+    p.tokens = a->tokens; p.sxb = a->sx;
+    p.accept_u = a->accept_u; p.sub = a->su;
+    p.sample_u = a->sample_u;
+    p.accepted = a->accepted; p.out = a->out;
+    p.B = (int)a->B; p.N = (int)a->N; p.V = (int)a->V;
+    const hipError_t e = launch_verify(p, a->dtype, reinterpret_cast<hipStream_t>(stream));
+    return e != hipSuccess ? hip_fail(e, "fpa_verify launch") : FPA_OK;
 }
 
 }  // extern "C"

@@ -1,0 +1,249 @@
+// fpa_cache.hip -- writing positions into the pages of a cache and reading them back.
+//
+// e4m3 rows.  The row of K or V of one position and head is kept as code * 2^e with
+//   e = clamp(ceil(log2(max |x| / 448)), -60, 60)   (-60 for a row of zeros),   code = e4m3(x * 2^-e),
+// rounded to nearest even, saturating.  A power of two costs an 8-bit floating-point format nothing (its
+// relative step is the same in every binade; only values 2^-15 below the row's maximum reach its subnormals),
+// scaling by it is exact, so the code is one rounding of the value itself, and the products take it out again
+// exactly: for K on the score, for V as an addition to the logit.  NaN stays NaN, an infinity saturates.
+//
+// Both kernels are passes over their bytes: one workgroup per (page, head, sequence), K rows moved in 16-byte
+// pieces, V turned in LDS.
+#include "fpa_common.h"
+#include "fpa_serve.h"
+
+namespace fpa {
+
+namespace {
+
+// Exponent of a row whose largest magnitude is amax (not NaN): amax = m 2^x with m in [0.5, 1) is at most
+// 448 * 2^e = 0.875 * 2^(9 + e) for e = x - 9 if m <= 0.875, else e = x - 8.  Subnormal amax: -60 either way.
+__device__ __forceinline__ int row_exp(float amax) {
+    const uint32_t b = __float_as_uint(amax);
+    const int x = (int)(b >> 23) - 126;
+    const int e = (b & 0x7fffffu) > 0x600000u ? x - 8 : x - 9;
+    return max(EXP_MIN, min(EXP_MAX, e));
+}
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+__device__ __forceinline__ bool is_nan(float x) { return (__float_as_uint(x) & 0x7fffffffu) > 0x7f800000u; }
+// |x| with NaN as 0.
+__device__ __forceinline__ float mag(float x) { return is_nan(x) ? 0.f : __uint_as_float(__float_as_uint(x) & 0x7fffffffu); }
+
+// Four scaled values as e4m3 codes.
+__device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) {
+    float x[4] = {a, b, c, d};
+    uint32_t nan = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        nan |= is_nan(x[i]) ? 0x7fu << (8 * i) : 0u;
+        x[i] = __builtin_amdgcn_fmed3f(x[i], -448.f, 448.f);
+    }
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], w, true);
+    return (uint32_t)w | nan;
+}
+
+// A lane's 16 bytes of one input row.
+template <typename TX> struct Piece {
+    static constexpr int N = 16 / sizeof(TX);
+    float x[N];
+    __device__ __forceinline__ void load(const TX *p) {
+        if constexpr (sizeof(TX) == 2) {
+            const h8 v = *reinterpret_cast<const h8 *>(p);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = (float)v[i];
+        } else {
+            const f32x4 v = *reinterpret_cast<const f32x4 *>(p);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = v[i];
+        }
+    }
+    // as the N values of the cache at dst
+    __device__ __forceinline__ void store(f16 *dst) const {
+        h8 v;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = (f16)x[i % N];
+        *reinterpret_cast<h8 *>(dst) = v;
+    }
+    __device__ __forceinline__ void store(float *dst) const { *reinterpret_cast<f32x4 *>(dst) = f32x4{x[0], x[1], x[2], x[3]}; }
+    __device__ __forceinline__ void store(e4m3 *dst) const {
+#pragma unroll
+        for (int i = 0; i < N; i += 4)
+            reinterpret_cast<uint32_t *>(dst)[i / 4] = codes4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+    }
+    // Scales the row that LPR neighbouring lanes hold together for e4m3; returns its exponent.
+    template <int LPR> __device__ __forceinline__ int scale() {
+        float m = 0.f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) m = fmaxf(m, mag(x[i]));
+#pragma unroll
+        for (int o = 1; o < LPR; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+        const int e = row_exp(m);
+        const float s = pow2(-e);
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] *= s;
+        return e;
+    }
+};
+
+template <typename TS> __device__ __forceinline__ float value(TS x, int e) {
+    if constexpr (sizeof(TS) == 1) {
+        const float v = __builtin_amdgcn_cvt_f32_fp8(x.code, 0);
+        return v * pow2(e);
+    } else {
+        return (float)x;
+    }
+}
+
+template <typename TX, typename TS, int D>
+__global__ __launch_bounds__(256) void fpa_append_kernel(MoveParams p) {
+    constexpr int N16 = Piece<TX>::N, LPR = D / N16, RPP = 256 / LPR;  // lanes of a row, rows of a pass
+    constexpr int LP = D + 16 / sizeof(TS);                              // pitch of the V tile in LDS
+    __shared__ __align__(16) TS tile[PG * LP];
+    const int tid = thread_x(), h = group_y(), b = group_z();
+    const int64_t start = p.start[b];
+    int64_t n = p.counts ? p.counts[b] : p.N;
+    n = n > p.N ? p.N : n;
+    if (start < 0) return;
+    const int64_t pg = start / PG + group_x();  // page of the sequence
+    const int lo = group_x() == 0 ? (int)(start % PG) : 0;
+    const int64_t left = start + n - pg * PG;  // positions of this page that are written, from its first
+    const int hi = left > PG ? PG : (int)left;
+    if (left <= lo || pg >= p.P) return;
+    const int page = p.table[(int64_t)b * p.stable + pg];
+    if ((uint32_t)page >= (uint64_t)p.c.n) return;  // no such page
+    const int64_t ph = (int64_t)page * p.c.H + h;
+    const int64_t i0 = pg * PG - start;  // token of the page's first position (may be negative)
+    const TX *k = static_cast<const TX *>(p.k) + (int64_t)b * p.sk.b + (int64_t)h * p.sk.h;
+    const TX *v = static_cast<const TX *>(p.v) + (int64_t)b * p.sv.b + (int64_t)h * p.sv.h;
+    TS *ck = static_cast<TS *>(p.c.k) + ph * PG * D;
+    TS *cv = static_cast<TS *>(p.c.v) + ph * PG * D;
+    const int col = tid % LPR * N16;
+    for (int r0 = 0; r0 < PG; r0 += RPP) {
+        const int r = r0 + tid / LPR;
+        if (r0 + RPP <= lo || r0 >= hi) continue;
+        const bool there = r >= lo && r < hi;
+        const int rr = min(max(r, lo), hi - 1);  // rows outside read a written one
+        Piece<TX> a, c;
+        a.load(k + (i0 + rr) * p.sk.t + col);
+        c.load(v + (i0 + rr) * p.sv.t + col);
+        if constexpr (sizeof(TS) == 1) {
+            const int ea = a.template scale<LPR>(), ec = c.template scale<LPR>();
+            if (there && tid % LPR == 0) {
+                p.c.k_exp[ph * PG + r] = (int8_t)ea;
+                p.c.v_exp[ph * PG + r] = (int8_t)ec;
+            }
+        }
+        if (there) {
+            a.store(ck + r * D + col);
+            c.store(tile + r * LP + col);
+        }
+    }
+    if (tid < PG) {
+        const bool there = tid >= lo && tid < hi;
+        float x = pinf();
+        if (there) {
+            x = p.phi[(int64_t)b * p.sphi.b + (int64_t)h * p.sphi.h + (i0 + tid) * p.sphi.t];
+            p.c.phi[ph * PG + tid] = x;
+            p.c.psi[ph * PG + tid] = p.psi[(int64_t)b * p.spsi.b + (int64_t)h * p.spsi.h + (i0 + tid) * p.spsi.t];
+        } else if (tid < lo) {
+            x = p.c.phi[ph * PG + tid];
+        }
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) x = fminf(x, __shfl_xor(x, o, 64));
+        if (tid == 0) p.c.phi_min[ph] = x;
+    }
+    __syncthreads();
+    // V^T: four positions of one feature per thread and step.
+    for (int e = tid; e < D * PG / 4; e += 256) {
+        const int d = e / (PG / 4), s = e % (PG / 4) * 4;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (s + i >= lo && s + i < hi) cv[d * PG + s + i] = tile[(s + i) * LP + d];
+    }
+}
+
+template <typename TX, typename TS, int D>
+__global__ __launch_bounds__(256) void fpa_read_kernel(MoveParams p) {
+    constexpr int LP = PG + 16 / sizeof(TS);
+    __shared__ __align__(16) TS tile[D * LP];
+    __shared__ int8_t ve[PG];
+    const int tid = thread_x(), h = group_y(), b = group_z();
+    int64_t start = p.start[b];
+    int64_t n = p.counts ? p.counts[b] : p.N;
+    n = n > p.N ? p.N : n;
+    bool there = start >= 0;
+    if (!there) start = 0;  // nothing to read: every row NaN
+    const int64_t pg = start / PG + group_x();
+    const int lo = group_x() == 0 ? (int)(start % PG) : 0;
+    const int64_t left = start + p.N - pg * PG;
+    const int hi = left > PG ? PG : (int)left;
+    if (left <= lo) return;
+    const int64_t i0 = pg * PG - start;
+    there = there && pg < p.P;
+    const int page = there ? p.table[(int64_t)b * p.stable + pg] : -1;
+    there = (uint32_t)page < (uint64_t)p.c.n && page >= 0;
+    const int64_t ph = there ? (int64_t)page * p.c.H + h : 0;
+    const TS *ck = static_cast<const TS *>(p.c.k) + ph * PG * D;
+    const TS *cv = static_cast<const TS *>(p.c.v) + ph * PG * D;
+    const int64_t row0 = ((int64_t)b * p.c.H + h) * p.N + i0;
+    for (int e = tid; e < D * PG && there; e += 256) tile[e / PG * LP + e % PG] = cv[e];
+    if (sizeof(TS) == 1 && tid < PG && there) ve[tid] = p.c.v_exp[ph * PG + tid];
+    __syncthreads();
+    const float nan = __uint_as_float(0x7fc00000u);
+    for (int e = lo * D + tid; e < hi * D; e += 256) {
+        const int r = e / D, d = e % D;
+        float kx = 0.f, vx = 0.f;
+        if (i0 + r < n) {
+            kx = vx = nan;
+            if (there) {
+                int ke = 0, vv = 0;
+                if constexpr (sizeof(TS) == 1) { ke = p.c.k_exp[ph * PG + r]; vv = ve[r]; }
+                kx = value(ck[e], ke);
+                vx = value(tile[d * LP + r], vv);
+            }
+        }
+        static_cast<TX *>(p.ko)[(row0 + r) * D + d] = (TX)kx;
+        static_cast<TX *>(p.vo)[(row0 + r) * D + d] = (TX)vx;
+    }
+    if (tid >= lo && tid < hi) {
+        const bool in = i0 + tid < n;
+        p.phio[row0 + tid] = !in ? 0.f : there ? p.c.phi[ph * PG + tid] : nan;
+        p.psio[row0 + tid] = !in ? 0.f : there ? p.c.psi[ph * PG + tid] : nan;
+    }
+}
+
+template <bool READ, typename TX, typename TS, int D> hipError_t launch_move_d(const MoveParams &p, hipStream_t s) {
+    const dim3 grid((p.N + PG - 2) / PG + 1, p.c.H, p.B);
+    if constexpr (READ)
+        hipLaunchKernelGGL((fpa_read_kernel<TX, TS, D>), grid, dim3(256), 0, s, p);
+    else
+        hipLaunchKernelGGL((fpa_append_kernel<TX, TS, D>), grid, dim3(256), 0, s, p);
+    return hipGetLastError();
+}
+
+template <bool READ, typename TX, typename TS> hipError_t launch_move_t(const MoveParams &p, hipStream_t s) {
+    switch (p.D) {
+        case 16: return launch_move_d<READ, TX, TS, 16>(p, s);
+        case 32: return launch_move_d<READ, TX, TS, 32>(p, s);
+        case 64: return launch_move_d<READ, TX, TS, 64>(p, s);
+        case 128: return launch_move_d<READ, TX, TS, 128>(p, s);
+        case 256: return launch_move_d<READ, TX, TS, 256>(p, s);
+    }
+    return hipErrorInvalidValue;
+}
+
+template <bool READ> hipError_t launch_move(const MoveParams &p, int dtype, int store, hipStream_t s) {
+    if (dtype == ST_F16 && store == ST_F16) return launch_move_t<READ, f16, f16>(p, s);
+    if (dtype == ST_F32 && store == ST_F32) return launch_move_t<READ, float, float>(p, s);
+    if (dtype == ST_F16 && store == ST_E4M3) return launch_move_t<READ, f16, e4m3>(p, s);
+    if (dtype == ST_F32 && store == ST_E4M3) return launch_move_t<READ, float, e4m3>(p, s);
+    return hipErrorInvalidValue;
+}
+
+}  // namespace
+
+hipError_t launch_append(const MoveParams &p, int dtype, int store, hipStream_t s) { return launch_move<false>(p, dtype, store, s); }
+hipError_t launch_read(const MoveParams &p, int dtype, int store, hipStream_t s) { return launch_move<true>(p, dtype, store, s); }
+
+}  // namespace fpa

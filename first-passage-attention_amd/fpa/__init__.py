@@ -6,6 +6,9 @@ Same surface as the reference module ``kernel`` of yliu-fort/first-passage-atten
 gfx950 kernels of ``libfpa.so`` (``"triton"`` is accepted as an alias so code written
 against the reference runs unchanged); ``impl="reference"`` is the dense PyTorch
 definition; ``impl=None`` picks ``"hip"`` for GPU tensors and ``"reference"`` otherwise.
+
+For models that answer there is, beside the reference's surface, a paged cache (``PagedCache``), attention against it
+(``cached_attention``, ``shared_prefix_attention``) and the verification of drafted tokens (``verify_drafts``).
 """
 import math
 
@@ -14,9 +17,12 @@ from torch import nn
 from torch.nn import functional as F
 
 from . import dense
+from .cache import PagedCache, cached_attention, shared_prefix_attention
 from .dense import first_passage_bias
+from .drafts import verify_drafts
 
-__all__ = ["first_passage_attention", "first_passage_bias", "Field", "FirstPassageAttention"]
+__all__ = ["first_passage_attention", "first_passage_bias", "Field", "FirstPassageAttention",
+           "PagedCache", "cached_attention", "shared_prefix_attention", "verify_drafts"]
 
 _HIP_NAMES = ("hip", "triton")
 

@@ -13,10 +13,10 @@ import torch
 
 from ._srchash import source_hash
 
-ABI_VERSION = 5
+ABI_VERSION = 6
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libfpa.so")
 
-FPA_F16, FPA_F32 = 0, 1
+FPA_F16, FPA_F32, FPA_E4M3 = 0, 1, 2
 FPA_OK, FPA_ERR_INVALID, FPA_ERR_UNSUPPORTED, FPA_ERR_HIP = 0, 1, 2, 3
 FPA_FWD_STATS, FPA_FWD_MAIN, FPA_FWD_MERGE = 1, 2, 4
 FPA_BWD_DELTA, FPA_BWD_KEYS, FPA_BWD_QUERIES, FPA_BWD_PHI, FPA_BWD_BETA = 1, 2, 4, 8, 16
@@ -70,6 +70,47 @@ class FpaFieldBwdArgs(ctypes.Structure):
                 ("dx", _vp), ("sdx", _S2), ("dweight", _vp), ("dbias", _vp), ("workspace", _vp)]
 
 
+class FpaPages(ctypes.Structure):
+    _fields_ = [("pages", _i64), ("H", _i64), ("D", _i64), ("store", ctypes.c_int32),
+                ("k", _vp), ("v", _vp), ("phi", _vp), ("psi", _vp), ("phi_min", _vp), ("k_exp", _vp), ("v_exp", _vp)]
+
+
+class FpaAppendArgs(ctypes.Structure):
+    _fields_ = [("cache", FpaPages), ("B", _i64), ("N", _i64), ("P", _i64), ("dtype", ctypes.c_int32),
+                ("k", _vp), ("sk", _S4), ("v", _vp), ("sv", _S4), ("phi", _vp), ("sphi", _S3), ("psi", _vp), ("spsi", _S3),
+                ("table", _vp), ("stable", _i64), ("start", _vp), ("counts", _vp)]
+
+
+class FpaReadArgs(ctypes.Structure):
+    _fields_ = [("cache", FpaPages), ("B", _i64), ("N", _i64), ("P", _i64), ("dtype", ctypes.c_int32),
+                ("k", _vp), ("v", _vp), ("phi", _vp), ("psi", _vp),
+                ("table", _vp), ("stable", _i64), ("start", _vp), ("counts", _vp)]
+
+
+class FpaAttendArgs(ctypes.Structure):
+    _fields_ = [("cache", FpaPages), ("B", _i64), ("N", _i64), ("P", _i64), ("dtype", ctypes.c_int32),
+                ("q", _vp), ("sq", _S4), ("o", _vp), ("so", _S4), ("beta", _vp),
+                ("table", _vp), ("stable", _i64), ("lengths", _vp), ("prefix", _vp), ("prefix_length", _i64),
+                ("workspace", _vp)]
+
+
+class FpaVerifyArgs(ctypes.Structure):
+    _fields_ = [("B", _i64), ("N", _i64), ("V", _i64), ("dtype", ctypes.c_int32),
+                ("target", _vp), ("st", _S2), ("draft", _vp), ("sd", _S2), ("tokens", _vp), ("sx", _i64),
+                ("accept_u", _vp), ("su", _i64), ("sample_u", _vp), ("accepted", _vp), ("out", _vp)]
+
+
+# Their byte images, as above; a cache's own part is packed once and kept with it.
+PAGES_PACK = struct.Struct("=qqqi4x" + "q" * 7)
+_CACHE = f"={PAGES_PACK.size}sqqqi4x"
+APPEND_PACK = struct.Struct(_CACHE + "q4q" * 2 + "q3q" * 2 + "qqqq")
+READ_PACK = struct.Struct(_CACHE + "qqqq" + "qqqq")
+ATTEND_PACK = struct.Struct(_CACHE + "q4q" * 2 + "q" + "qqq" + "qq" + "q")
+VERIFY_PACK = struct.Struct("=qqqi4x" + "q2q" * 2 + "qq" * 2 + "qqq")
+assert [x.size for x in (PAGES_PACK, APPEND_PACK, READ_PACK, ATTEND_PACK, VERIFY_PACK)] == [
+    ctypes.sizeof(x) for x in (FpaPages, FpaAppendArgs, FpaReadArgs, FpaAttendArgs, FpaVerifyArgs)]
+
+
 class FpaError(RuntimeError):
     """A failed libfpa call (status code and message of fpa_last_error)."""
 
@@ -110,6 +151,12 @@ def lib():
     L.fpa_field_fwd.argtypes = [ctypes.POINTER(FpaFieldFwdArgs), _vp]
     L.fpa_field_bwd.restype = ctypes.c_int
     L.fpa_field_bwd.argtypes = [ctypes.POINTER(FpaFieldBwdArgs), _vp]
+    for name, args in (("fpa_cache_append", FpaAppendArgs), ("fpa_cache_read", FpaReadArgs),
+                       ("fpa_attend", FpaAttendArgs), ("fpa_verify", FpaVerifyArgs)):
+        getattr(L, name).restype = ctypes.c_int
+        getattr(L, name).argtypes = [ctypes.POINTER(args), _vp]
+    L.fpa_attend_workspace_bytes.restype = _i64
+    L.fpa_attend_workspace_bytes.argtypes = [_i64] * 6
     if L.fpa_abi_version() != ABI_VERSION:
         raise RuntimeError(f"libfpa.so ABI {L.fpa_abi_version()} != {ABI_VERSION}: rebuild it")
     L.fpa_source_hash.restype = ctypes.c_char_p

@@ -39,6 +39,9 @@ extern "C" {
 /* dtype of q, k, v, o, do, dq, dk, dv */
 #define FPA_F16 0
 #define FPA_F32 1
+/* of the pages of a cache only: 8-bit floating point (4 exponent and 3 mantissa bits, no infinities),
+ * each row with a power of two of its own */
+#define FPA_E4M3 2
 
 /* phase bits (FpaFwdArgs.phases / FpaBwdArgs.phases) */
 #define FPA_FWD_STATS 1    /* block statistics of phi                      */
@@ -186,6 +189,104 @@ int fpa_bwd(const FpaBwdArgs *args, void *stream);
  * serialise them.  Allocates nothing (no hipMalloc or allocating library routine).            */
 #define FPA_NOALLOC_SCRATCH_BYTES (64ll << 20)
 int fpa_bwd_noalloc(const FpaBwdArgs *args, void *stream);
+
+/* ---------------------------------------------------------------------------
+ * Serving: a paged cache, attention of new tokens against it, drafted tokens.  No counterpart in the
+ * reference, which has the training forward and backward only.
+ *
+ * A page holds 64 positions of every head.  Tables name a sequence's pages in order (int32; entries behind
+ * its last page are not read); lengths, starts and counts are int32 in device memory.  Nothing is checked
+ * that only the device knows: a page outside the pool is never touched (appends to it are dropped; what is read
+ * from it, and every attention row that would need it, is NaN), and so is a position outside the table.
+ * --------------------------------------------------------------------------- */
+
+/* The pages, every buffer contiguous and 16-byte aligned. */
+typedef struct {
+    int64_t pages, H, D;
+    int32_t store;      /* FPA_F16, FPA_F32 or FPA_E4M3 */
+    void *k;            /* (pages, H, 64, D) */
+    void *v;            /* (pages, H, D, 64): V of a page transposed */
+    float *phi, *psi;   /* (pages, H, 64) */
+    float *phi_min;     /* (pages, H): min of phi over the page's written positions */
+    int8_t *k_exp;      /* (pages, H, 64), FPA_E4M3 only: a row of k or v is its codes times 2^exp */
+    int8_t *v_exp;
+} FpaPages;
+
+/* Writes positions start[b] + i, i < counts[b] (at most N; N without counts) of B sequences.  k, v: (B, H, N, D)
+ * with a unit d stride and 16-byte aligned rows, of the pages' type, or fp16 or fp32 for FPA_E4M3; phi, psi
+ * (B, H, N).  Positions of one page must not be written by two sequences of a call.
+ * e4m3: exp = clamp(ceil(log2(max |row| / 448)), -60, 60), -60 for a row of zeros; codes are rounded to nearest
+ * even and saturate, NaN stays NaN.                                                              */
+typedef struct {
+    FpaPages cache;
+    int64_t B, N, P;    /* table is (B, P) */
+    int32_t dtype;      /* of k and v: FPA_F16 or FPA_F32 */
+    const void *k;  int64_t sk[4];
+    const void *v;  int64_t sv[4];
+    const float *phi; int64_t sphi[3];
+    const float *psi; int64_t spsi[3];
+    const int32_t *table; int64_t stable;  /* row stride of table, in elements */
+    const int32_t *start;
+    const int32_t *counts;                 /* or NULL */
+} FpaAppendArgs;
+int fpa_cache_append(const FpaAppendArgs *args, void *stream);
+
+/* Reads the same positions back into k, v (B, H, N, D) and phi, psi (B, H, N), contiguous; zero where
+ * i >= counts[b].  dtype: the pages' type, or either for FPA_E4M3.                                */
+typedef struct {
+    FpaPages cache;
+    int64_t B, N, P;
+    int32_t dtype;
+    void *k, *v;
+    float *phi, *psi;
+    const int32_t *table; int64_t stable;
+    const int32_t *start;
+    const int32_t *counts;
+} FpaReadArgs;
+int fpa_cache_read(const FpaReadArgs *args, void *stream);
+
+/* First Passage Attention of the last N positions of B sequences, lengths[b] positions each (the N new ones
+ * among them), against their pages: query i stands at position t = lengths[b] - N + i and attends to s <= t;
+ * rows with t < 0 are zero.  With prefix_length > 0 every sequence continues one prefix of that many
+ * positions on the pages prefix[0 .. ceil(prefix_length / 64)): rows attend to all of it too, and to phi across
+ * the border; lengths and table still count the sequence's own positions alone.
+ * q: (B, H, N, D), unit d stride, 16-byte aligned rows, fp16 or fp32 (the pages' type unless that is FPA_E4M3);
+ * o: likewise, any alignment.                                                                      */
+typedef struct {
+    FpaPages cache;
+    int64_t B, N, P;
+    int32_t dtype;
+    const void *q;  int64_t sq[4];
+    void *o;        int64_t so[4];
+    const float *beta;                     /* (H,) */
+    const int32_t *table; int64_t stable;
+    const int32_t *lengths;
+    const int32_t *prefix;                 /* or NULL */
+    int64_t prefix_length;
+    void *workspace;                       /* fpa_attend_workspace_bytes(), 256-byte aligned */
+} FpaAttendArgs;
+int64_t fpa_attend_workspace_bytes(int64_t B, int64_t H, int64_t N, int64_t D, int64_t P, int64_t prefix_length);
+int fpa_attend(const FpaAttendArgs *args, void *stream);
+
+/* Verifies N drafted tokens of B sequences.  target: probabilities (B, N + 1, V), draft: (B, N, V) or NULL for
+ * drafts that count as certain; unit stride over V.  Draft i is accepted while
+ * accept_u[b, i] * draft[b, i, x_i] < target[b, i, x_i]; a token outside 0 .. V - 1 ends the drafts.  The next token is the
+ * lowest v whose running sum of weights passes sample_u[b] times their sum, the weights being
+ * max(target - draft, 0) of the rejected position's row, or the target's row where that is zero, where all
+ * drafts are accepted and where they end (-1 if that row has no positive finite sum).  accepted: (B,); out: (B, N + 1),
+ * the accepted drafts, the next token, then -1.                                                */
+typedef struct {
+    int64_t B, N, V;
+    int32_t dtype;      /* of target and draft: FPA_F16 or FPA_F32 */
+    const void *target; int64_t st[2];     /* strides of b and position */
+    const void *draft;  int64_t sd[2];
+    const int64_t *tokens; int64_t sx;     /* (B, N), row stride sx */
+    const float *accept_u; int64_t su;     /* (B, N), row stride su, in [0, 1) */
+    const float *sample_u;                 /* (B,), in [0, 1) */
+    int64_t *accepted;
+    int64_t *out;                          /* contiguous */
+} FpaVerifyArgs;
+int fpa_verify(const FpaVerifyArgs *args, void *stream);
 
 /* Message of the last failed call on this host thread ("" if none). */
 const char *fpa_last_error(void);
