@@ -446,10 +446,11 @@ struct AttendPlan {
     int chunk, nchunk, pchunk = 1, npchunk = 0;
     int64_t ml, total;  // float offset of the statistics, bytes
 };
-AttendPlan attend_plan(int64_t B, int64_t H, int64_t N, int64_t D, int64_t P, int64_t PL) {
+AttendPlan attend_plan(int64_t B, int64_t H, int64_t N, int64_t D, int64_t P, int64_t PL, int32_t dtype) {
     AttendPlan a;
-    attend_parts(B * H * ((N + 15) / 16), P, a.chunk, a.nchunk);
-    if (PL > 0) attend_parts(H * ((B * N + 15) / 16), (PL + PG - 1) / PG, a.pchunk, a.npchunk);
+    const int64_t rows = attend_rows(B * N, (int)D, dtype);
+    attend_parts(B * H * ((N + 15) / 16), P, (int)D, a.chunk, a.nchunk);
+    if (PL > 0) attend_parts(H * ((B * N + rows - 1) / rows), (PL + PG - 1) / PG, (int)D, a.pchunk, a.npchunk);
     const int64_t slots = (a.nchunk <= 1 && a.npchunk == 0) ? 0 : (int64_t)(a.nchunk + a.npchunk) * B * H * N;
     a.ml = align64(slots * D);
     a.total = (a.ml + align64(slots * 2)) * (int64_t)sizeof(float);
@@ -497,9 +498,9 @@ int fpa_cache_read(const FpaReadArgs *a, void *stream) {
     return e != hipSuccess ? hip_fail(e, "fpa_cache_read launch") : FPA_OK;
 }
 
-int64_t fpa_attend_workspace_bytes(int64_t B, int64_t H, int64_t N, int64_t D, int64_t P, int64_t prefix_length) {
+int64_t fpa_attend_workspace_bytes(int64_t B, int64_t H, int64_t N, int64_t D, int64_t P, int64_t prefix_length, int32_t dtype) {
     if (B < 1 || H < 1 || N < 1 || D < 1 || P < 1) return 0;
-    return attend_plan(B, H, N, D, P, prefix_length).total;
+    return attend_plan(B, H, N, D, P, prefix_length, dtype).total;
 }
 
 int fpa_attend(const FpaAttendArgs *a, void *stream) {
@@ -514,11 +515,12 @@ int fpa_attend(const FpaAttendArgs *a, void *stream) {
         return fail(FPA_ERR_INVALID, "prefix_length must be between 0 and " + std::to_string((int64_t)MAX_NB * G));
     if (a->prefix_length > 0 && !a->prefix) return fail(FPA_ERR_INVALID, "prefix is NULL");
     const int64_t H = a->cache.H, D = a->cache.D;
-    const AttendPlan pl = attend_plan(a->B, H, a->N, D, a->P, a->prefix_length);
+    const AttendPlan pl = attend_plan(a->B, H, a->N, D, a->P, a->prefix_length, a->dtype);
     if (pl.total > 0 && (a->workspace == nullptr || (reinterpret_cast<uintptr_t>(a->workspace) & 255) != 0))
         return fail(FPA_ERR_INVALID, "workspace must be non-NULL and 256-byte aligned");
-    // One workgroup per part and row tile, one merge thread per output element: grids below 2^31.
-    if ((double)a->B * H * a->N * (pl.nchunk + pl.npchunk) >= 2147483648.0 || (double)a->B * H * a->N * D / 256 >= 2147483647.0)
+    if (!a->counts || (reinterpret_cast<uintptr_t>(a->counts) & 3) != 0) return fail(FPA_ERR_INVALID, "counts must be non-NULL");
+    // One workgroup per part and row tile: a grid below 2^31.
+    if ((double)a->B * H * a->N * (pl.nchunk + pl.npchunk + 8) >= 2147483648.0)
         return fail(FPA_ERR_UNSUPPORTED, "B * H * N is too large");
     AttendParams p = {};
     p.c = pages_of(a->cache);
@@ -528,11 +530,18 @@ int fpa_attend(const FpaAttendArgs *a, void *stream) {
     p.table = a->table; p.stable = a->stable; p.lengths = a->lengths; p.prefix = a->prefix;
     p.part = static_cast<float *>(a->workspace);
     p.ml = p.part + pl.ml;
+    p.counts = a->counts;
     p.B = (int)a->B; p.N = (int)a->N; p.P = (int)a->P; p.PL = (int)a->prefix_length;
     p.chunk = pl.chunk; p.nchunk = pl.nchunk; p.pchunk = pl.pchunk; p.npchunk = pl.npchunk;
     p.sc2 = LOG2E / sqrtf((float)D);
     const hipError_t e = launch_attend(p, a->dtype, a->cache.store, (int)D, reinterpret_cast<hipStream_t>(stream));
     return e != hipSuccess ? hip_fail(e, "fpa_attend launch") : FPA_OK;
+}
+
+int64_t fpa_verify_workspace_bytes(int64_t B, int64_t V) {
+    if (B < 1 || V < 1) return 0;
+    const int64_t span = verify_span(B, V), spans = (V + span - 1) / span;
+    return (B * spans * 16 + B * 4 + 255) / 256 * 256;
 }
 
 int fpa_verify(const FpaVerifyArgs *a, void *stream) {
@@ -544,7 +553,13 @@ int fpa_verify(const FpaVerifyArgs *a, void *stream) {
         return fail(FPA_ERR_UNSUPPORTED, "B must be at most 65535, N at most 2^20 and V at most 2^30");
     if (!a->target || !a->sample_u || !a->accepted || !a->out || (a->N > 0 && (!a->tokens || !a->accept_u)))
         return fail(FPA_ERR_INVALID, "target, tokens, accept_u, sample_u, accepted and out must be non-NULL");
+    if (a->workspace == nullptr || (reinterpret_cast<uintptr_t>(a->workspace) & 255) != 0)
+        return fail(FPA_ERR_INVALID, "workspace must be non-NULL and 256-byte aligned");
     VerifyParams p = {};
+    p.span = verify_span(a->B, a->V);
+    p.spans = (int)((a->V + p.span - 1) / p.span);
+    p.sums = static_cast<double *>(a->workspace);
+    p.none = reinterpret_cast<int32_t *>(p.sums + a->B * p.spans * 2);
     p.target = a->target; p.stb = a->st[0]; p.stn = a->st[1];
     p.draft = a->N > 0 ? a->draft : nullptr; p.sdb = a->sd[0]; p.sdn = a->sd[1];
     p.tokens = a->tokens; p.sxb = a->sx;

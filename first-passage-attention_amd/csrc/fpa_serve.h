@@ -54,6 +54,7 @@ struct AttendParams {
     const int32_t *lengths;
     const int32_t *prefix;
     float *part, *ml;      // per part and row: O (D floats), then its running maximum and sum
+    int32_t *counts;       // (B, H): parts done, 0 before and after every launch
     int B, N, P;
     int PL;                // positions of the shared prefix (0: none)
     int chunk, nchunk;     // pages of a part, parts at most, of a sequence's own pages
@@ -68,14 +69,20 @@ struct VerifyParams {
     const float *accept_u; int64_t sub;
     const float *sample_u;
     int64_t *accepted, *out;
+    double *sums;  // (B, spans, 2): of each span's tokens
+    int32_t *none; // (B,): no token at the rejected position
     int B, N, V;
+    int span, spans;
 };
 
 hipError_t launch_append(const MoveParams &p, int dtype, int store, hipStream_t s);
 hipError_t launch_read(const MoveParams &p, int dtype, int store, hipStream_t s);
 hipError_t launch_attend(const AttendParams &p, int dtype, int store, int D, hipStream_t s);
 // Pages of a part and parts at most, for rows of at most `pages` pages; `items` counts the parts' other axes.
-void attend_parts(int64_t items, int64_t pages, int &chunk, int &nchunk);
+int attend_rows(int64_t rows, int D, int dtype);  // rows of a tile of the prefix
+void attend_parts(int64_t items, int64_t pages, int D, int &chunk, int &nchunk);
+// Tokens of a span.
+int verify_span(int64_t B, int64_t V);
 hipError_t launch_verify(const VerifyParams &p, int dtype, hipStream_t s);
 
 }  // namespace fpa

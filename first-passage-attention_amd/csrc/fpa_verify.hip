@@ -16,25 +16,25 @@ namespace fpa {
 
 namespace {
 
-constexpr int VT = 1024, VW = VT / 64;
+constexpr int VT = 256, VW = VT / 64;
 
 template <typename T> __device__ __forceinline__ double prob(const T *row, int64_t v) { return (double)(float)row[v]; }
 
 __device__ __forceinline__ bool positive(double x) {  // > 0 and finite
     return x > 0.0 && x <= 1.7976931348623157e308;
 }
+__device__ __forceinline__ double above(double w) { return w < 0.0 ? 0.0 : w; }  // NaN stays: the row has no sum then
 
-// Weight of token v: p, or what it has more than q.
-template <typename T, bool Q> __device__ __forceinline__ double weight(const T *p, const T *q, int64_t x, int64_t v) {
-    double w = prob(p, v);
-    if constexpr (Q) {
-        if (q)
-            w -= prob(q, v);
-        else if (v == x)
-            w = 0.0;
+// What is drawn from: row n of the target, less the draft's row unless `whole`.
+template <typename T> struct Row {
+    const T *p, *q;
+    int64_t x;  // the drafted token, which has weight 0 where the drafts have no probabilities
+    __device__ __forceinline__ double target(int64_t v) const { return above(prob(p, v)); }
+    __device__ __forceinline__ double rest(int64_t v) const {  // what the target has more than the draft
+        if (q) return above(prob(p, v) - prob(q, v));
+        return v == x ? 0.0 : above(prob(p, v));
     }
-    return w < 0.0 ? 0.0 : w;  // NaN stays: the row has no sum then
-}
+};
 
 __device__ __forceinline__ double wave_sum(double x) {
 #pragma unroll
@@ -42,111 +42,212 @@ __device__ __forceinline__ double wave_sum(double x) {
     return x;
 }
 
-// The lowest v with sum_{v' <= v} w > r * sum w; -1 when the weights have no positive finite sum.
-template <typename T, bool Q>
-__device__ int64_t draw(const T *p, const T *q, int64_t x, int V, double r, double *seg, int *found) {
-    const int lane = thread_x() % 64, wave = thread_x() / 64;
-    const int per = (V + VW - 1) / VW, v0 = min(wave * per, V), v1 = min(v0 + per, V);
-    double s = 0.0;
-    for (int v = v0 + lane; v < v1; v += 64) s += weight<T, Q>(p, q, x, v);
-    s = wave_sum(s);
-    __syncthreads();  // seg and found are free
-    if (lane == 0) seg[wave] = s;
-    if (thread_x() == 0) *found = -1;
-    __syncthreads();
-    double total = 0.0;
-#pragma unroll
-    for (int w = 0; w < VW; ++w) total += seg[w];
-    if (!positive(total)) return -1;
-    // the first segment whose end passes the target, or the last with any weight
-    const double target = r * total;
-    double before = 0.0, at = 0.0;
-    int pick = -1, lastw = 0;
-    for (int w = 0; w < VW; ++w) {
-        if (seg[w] > 0.0) lastw = w;
-        if (pick < 0 && before + seg[w] > target) {
-            pick = w;
-            at = before;
-        }
-        before += seg[w];
-    }
-    if (pick < 0) {
-        pick = lastw;
-        at = before - seg[lastw];
-    }
-    if (wave == pick) {
-        int64_t token = -1, least = -1;  // least: the last token with weight, for sums that round below the target
-        for (int v = v0; v < v1 && token < 0; v += 64) {
-            const double w = v + lane < v1 ? weight<T, Q>(p, q, x, v + lane) : 0.0;
-            double c = w;
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) {
-                const double u = __shfl_up(c, o, 64);
-                if (lane >= o) c += u;
+// The first draft that is not accepted (N: none), by one wave; `none`: there is no token there.
+template <typename T> __device__ int first_rejected(const VerifyParams &a, const T *p, const T *q, const int64_t *x, const float *u, bool &none) {
+    const int lane = thread_x() % 64;
+    none = true;
+    for (int i0 = 0; i0 < a.N; i0 += 64) {
+        const int i = i0 + lane;
+        bool in = false, ok = false;
+        if (i < a.N) {
+            const int64_t t = x[i];
+            in = t >= 0 && t < a.V;
+            if (in) {
+                const double qx = q ? prob(q + (int64_t)i * a.sdn, t) : 1.0;
+                ok = (double)u[i] * qx < prob(p + (int64_t)i * a.stn, t);
             }
-            const uint64_t some = __ballot(w > 0.0), over = __ballot(w > 0.0 && at + c > target);
-            if (over) token = v + __builtin_ctzll(over);
-            if (some) least = v + 63 - __builtin_clzll(some);
-            at += __shfl(c, 63, 64);
         }
-        if (lane == 0) *found = (int)(token >= 0 ? token : least);
+        const uint64_t stop = __ballot(i < a.N && !ok), there = __ballot(in);
+        if (stop) {
+            const int k = __builtin_ctzll(stop);
+            none = (there >> k & 1) == 0;
+            return i0 + k;
+        }
     }
-    __syncthreads();
-    return *found;
+    return a.N;
 }
 
-template <typename T> __global__ __launch_bounds__(VT) void fpa_verify_kernel(VerifyParams a) {
-    __shared__ double seg[VW];
-    __shared__ int found, first, none;
-    const int b = group_x(), lane = thread_x() % 64;
+// Sums of each span of a sequence's row: sums[b][span] = (rest, target).  Every workgroup finds the rejected
+// position for itself; the first of a sequence keeps it for the second kernel.
+template <typename T> __global__ __launch_bounds__(VT) void fpa_verify_sum_kernel(VerifyParams a) {
+    __shared__ double part[2 * VW];
+    __shared__ int first, none;
+    const int b = group_y(), span = group_x(), lane = thread_x() % 64, wave = thread_x() / 64;
     const T *p = static_cast<const T *>(a.target) + (int64_t)b * a.stb;
     const T *q = a.draft ? static_cast<const T *>(a.draft) + (int64_t)b * a.sdb : nullptr;
     const int64_t *x = a.tokens + (int64_t)b * a.sxb;
-    const float *u = a.accept_u + (int64_t)b * a.sub;
-    if (thread_x() < 64) {  // the first draft that is not accepted, and whether there is a token there at all
-        int n = a.N, end = 1;
-        for (int i0 = 0; i0 < a.N; i0 += 64) {
-            const int i = i0 + lane;
-            bool in = false, ok = false;
-            if (i < a.N) {
-                const int64_t t = x[i];
-                in = t >= 0 && t < a.V;
-                if (in) {
-                    const double qx = q ? prob(q + (int64_t)i * a.sdn, t) : 1.0;
-                    ok = (double)u[i] * qx < prob(p + (int64_t)i * a.stn, t);
-                }
-            }
-            const uint64_t stop = __ballot(i < a.N && !ok), there = __ballot(in);
-            if (stop) {
-                const int k = __builtin_ctzll(stop);
-                n = i0 + k;
-                end = (there >> k & 1) == 0;
-                break;
-            }
-        }
+    if (wave == 0) {
+        bool no;
+        const int n = first_rejected(a, p, q, x, a.accept_u + (int64_t)b * a.sub, no);
         if (lane == 0) {
             first = n;
-            none = end;
+            none = no;
+            if (span == 0) {
+                a.accepted[b] = n;
+                a.none[b] = no;
+            }
         }
     }
     __syncthreads();
     const int n = first;
-    const T *pr = p + (int64_t)n * a.stn;
-    const double r = (double)a.sample_u[b];
+    const bool no = none;
+    const Row<T> row = {p + (int64_t)n * a.stn, q && !no ? q + (int64_t)n * a.sdn : nullptr, no ? -1 : x[n]};
+    const int v0 = span * a.span, v1 = min(v0 + a.span, a.V);
+    double rest = 0.0, target = 0.0;
+#pragma unroll 4
+    for (int v = v0 + thread_x(); v < v1; v += VT) {
+        rest += row.rest(v);
+        target += row.target(v);
+    }
+    rest = wave_sum(rest);
+    target = wave_sum(target);
+    if (lane == 0) {
+        part[2 * wave] = rest;
+        part[2 * wave + 1] = target;
+    }
+    __syncthreads();
+    if (thread_x() < 2) {
+        double s = part[thread_x()];
+#pragma unroll
+        for (int w = 1; w < VW; ++w) s += part[2 * w + thread_x()];
+        a.sums[2 * ((int64_t)b * a.spans + span) + thread_x()] = s;
+    }
+}
+
+// Inclusive sums of one value per thread in thread order; total gets the sum of all.
+__device__ __forceinline__ double block_sums(double x, double *part, double &total) {
+    const int lane = thread_x() % 64, wave = thread_x() / 64;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const double u = __shfl_up(x, o, 64);
+        if (lane >= o) x += u;
+    }
+    __syncthreads();  // part is free
+    if (lane == 63) part[wave] = x;
+    __syncthreads();
+    double before = 0.0;
+    total = 0.0;
+#pragma unroll
+    for (int w = 0; w < VW; ++w) {
+        if (w < wave) before += part[w];
+        total += part[w];
+    }
+    return before + x;
+}
+// The lowest thread for which `over` holds, else the highest for which `some` holds, else -1.
+__device__ __forceinline__ int block_pick(bool over, bool some, int *pick) {
+    __syncthreads();
+    if (thread_x() == 0) {
+        pick[0] = VT;
+        pick[1] = -1;
+    }
+    __syncthreads();
+    const uint64_t o = __ballot(over), s = __ballot(some);
+    if (thread_x() % 64 == 0) {
+        const int t0 = thread_x();
+        if (o) atomicMin(&pick[0], t0 + __builtin_ctzll(o));
+        if (s) atomicMax(&pick[1], t0 + 63 - __builtin_clzll(s));
+    }
+    __syncthreads();
+    return pick[0] < VT ? pick[0] : pick[1];
+}
+
+// Draws the token: the span that the target falls into, then the token in the span; sums that round below the target
+// fall to the last one with any weight.
+template <typename T> __global__ __launch_bounds__(VT) void fpa_verify_draw_kernel(VerifyParams a) {
+    __shared__ double part[VW], at;
+    __shared__ int pick[2], found;
+    const int b = group_x(), tid = thread_x();
+    const int64_t *x = a.tokens + (int64_t)b * a.sxb;
+    const int n = (int)a.accepted[b];
+    const bool no = a.none[b] != 0;
+    const T *q = a.draft ? static_cast<const T *>(a.draft) + (int64_t)b * a.sdb : nullptr;
+    const Row<T> row = {static_cast<const T *>(a.target) + (int64_t)b * a.stb + (int64_t)n * a.stn,
+                        q && !no ? q + (int64_t)n * a.sdn : nullptr, no ? -1 : x[n]};
+    const double *sums = a.sums + 2 * (int64_t)b * a.spans;
+    // a thread's spans: EACH neighbouring ones
+    const int each = (a.spans + VT - 1) / VT, s0 = min(tid * each, a.spans), s1 = min(s0 + each, a.spans);
+    double rest = 0.0, target = 0.0;
+    for (int s = s0; s < s1; ++s) {
+        rest += sums[2 * s];
+        target += sums[2 * s + 1];
+    }
+    double total;
+    double upto = block_sums(rest, part, total);
+    const bool use_rest = !no && positive(total);
+    if (!use_rest) upto = block_sums(target, part, total);
     int64_t token = -1;
-    if (!none) token = draw<T, true>(pr, q ? q + (int64_t)n * a.sdn : nullptr, x[n], a.V, r, seg, &found);
-    if (token < 0) token = draw<T, false>(pr, nullptr, -1, a.V, r, seg, &found);
-    for (int i = thread_x(); i <= a.N; i += VT) a.out[(int64_t)b * (a.N + 1) + i] = i < n ? x[i] : i == n ? token : -1;
-    if (thread_x() == 0) a.accepted[b] = n;
+    if (positive(total)) {
+        const double goal = (double)a.sample_u[b] * total, mine = use_rest ? rest : target;
+        int who = block_pick(mine > 0.0 && upto > goal, mine > 0.0, pick);
+        if (tid == who) {
+            double run = upto - mine;
+            if (s0 == 0) run = 0.0;
+            int s = s0, last = s0;
+            double last_run = run;
+            for (; s < s1; ++s) {
+                const double w = sums[2 * s + !use_rest];
+                if (w > 0.0) {
+                    last = s;
+                    last_run = run;
+                    if (run + w > goal) break;
+                }
+                run += w;
+            }
+            found = last;
+            at = last_run;
+        }
+        __syncthreads();
+        const int v0 = found * a.span, v1 = min(v0 + a.span, a.V);
+        const int per = (v1 - v0 + VT - 1) / VT, t0 = min(v0 + tid * per, v1), t1 = min(t0 + per, v1);
+        double w = 0.0;
+        for (int v = t0; v < t1; ++v) w += use_rest ? row.rest(v) : row.target(v);
+        const double base = at;
+        double all;
+        const double end = base + block_sums(w, part, all);
+        who = block_pick(w > 0.0 && end > goal, w > 0.0, pick);
+        if (tid == who) {
+            double run = end - w;
+            int last = -1;
+            for (int v = t0; v < t1; ++v) {
+                const double y = use_rest ? row.rest(v) : row.target(v);
+                run += y;
+                if (y > 0.0) {
+                    last = v;
+                    if (run > goal) break;
+                }
+            }
+            found = last;
+        }
+        __syncthreads();
+        token = found;
+    }
+    for (int i = tid; i <= a.N; i += VT) a.out[(int64_t)b * (a.N + 1) + i] = i < n ? x[i] : i == n ? token : -1;
 }
 
 }  // namespace
 
+int verify_span(int64_t B, int64_t V) {
+    // Spans of a multiple of 1024 tokens, about 2048 workgroups in all (eight on a CU, 4096 tokens each at the most
+    // common sizes).  B64 V128003 fp32: see the table beside fpa_verify_sum_kernel.
+    int64_t per = (B * V + 2047) / 2048;
+    per = per < V ? per : V;
+    per = (per + 1023) / 1024 * 1024;
+    return (int)per;
+}
+
 hipError_t launch_verify(const VerifyParams &p, int dtype, hipStream_t s) {
-    if (dtype == ST_F16)
-        hipLaunchKernelGGL((fpa_verify_kernel<f16>), dim3(p.B), dim3(VT), 0, s, p);
-    else
-        hipLaunchKernelGGL((fpa_verify_kernel<float>), dim3(p.B), dim3(VT), 0, s, p);
+    if (dtype == ST_F16) {
+        hipLaunchKernelGGL((fpa_verify_sum_kernel<f16>), dim3(p.spans, p.B), dim3(VT), 0, s, p);
+        hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+        hipLaunchKernelGGL((fpa_verify_draw_kernel<f16>), dim3(p.B), dim3(VT), 0, s, p);
+    } else {
+        hipLaunchKernelGGL((fpa_verify_sum_kernel<float>), dim3(p.spans, p.B), dim3(VT), 0, s, p);
+        hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+        hipLaunchKernelGGL((fpa_verify_draw_kernel<float>), dim3(p.B), dim3(VT), 0, s, p);
+    }
     return hipGetLastError();
 }
 

@@ -75,11 +75,16 @@ class FwdBuffers:
 _WS_CACHE = {}
 
 
+def _stream_key(dev):
+    i = dev.index if dev.index is not None else torch.cuda.current_device()
+    return i, _lib.stream_of(dev).value
+
+
 def workspace(dev, nbytes):
     """A uint8 device tensor of at least nbytes for one forward or backward call on the current stream."""
     if torch.cuda.is_current_stream_capturing():
         return torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    key = (dev.index if dev.index is not None else torch.cuda.current_device(), torch.cuda.current_stream(dev).cuda_stream)
+    key = _stream_key(dev)
     ws = _WS_CACHE.get(key)
     if ws is None or ws.numel() < nbytes:
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
@@ -90,6 +95,23 @@ def workspace(dev, nbytes):
 def release_workspaces():
     """Drop the cached backward scratch (torch's allocator gets the memory back)."""
     _WS_CACHE.clear()
+    _COUNT_CACHE.clear()
+
+
+# Counters that a launch finds and leaves at zero, kept like the scratch: calls on one stream run in order.  A captured
+# graph gets its own, with the fill that zeroes them before every replay.
+_COUNT_CACHE = {}
+
+
+def counters(dev, n):
+    """An int32 device tensor of at least n zeros for one call on the current stream."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.zeros(n, dtype=torch.int32, device=dev)
+    key = _stream_key(dev)
+    c = _COUNT_CACHE.get(key)
+    if c is None or c.numel() < n:
+        c = _COUNT_CACHE[key] = torch.zeros(max(n, 4096), dtype=torch.int32, device=dev)
+    return c
 
 
 class BwdBuffers:

@@ -91,13 +91,14 @@ class FpaAttendArgs(ctypes.Structure):
     _fields_ = [("cache", FpaPages), ("B", _i64), ("N", _i64), ("P", _i64), ("dtype", ctypes.c_int32),
                 ("q", _vp), ("sq", _S4), ("o", _vp), ("so", _S4), ("beta", _vp),
                 ("table", _vp), ("stable", _i64), ("lengths", _vp), ("prefix", _vp), ("prefix_length", _i64),
-                ("workspace", _vp)]
+                ("workspace", _vp), ("counts", _vp)]
 
 
 class FpaVerifyArgs(ctypes.Structure):
     _fields_ = [("B", _i64), ("N", _i64), ("V", _i64), ("dtype", ctypes.c_int32),
                 ("target", _vp), ("st", _S2), ("draft", _vp), ("sd", _S2), ("tokens", _vp), ("sx", _i64),
-                ("accept_u", _vp), ("su", _i64), ("sample_u", _vp), ("accepted", _vp), ("out", _vp)]
+                ("accept_u", _vp), ("su", _i64), ("sample_u", _vp), ("accepted", _vp), ("out", _vp),
+                ("workspace", _vp)]
 
 
 # Their byte images, as above; a cache's own part is packed once and kept with it.
@@ -105,8 +106,8 @@ PAGES_PACK = struct.Struct("=qqqi4x" + "q" * 7)
 _CACHE = f"={PAGES_PACK.size}sqqqi4x"
 APPEND_PACK = struct.Struct(_CACHE + "q4q" * 2 + "q3q" * 2 + "qqqq")
 READ_PACK = struct.Struct(_CACHE + "qqqq" + "qqqq")
-ATTEND_PACK = struct.Struct(_CACHE + "q4q" * 2 + "q" + "qqq" + "qq" + "q")
-VERIFY_PACK = struct.Struct("=qqqi4x" + "q2q" * 2 + "qq" * 2 + "qqq")
+ATTEND_PACK = struct.Struct(_CACHE + "q4q" * 2 + "q" + "qqq" + "qq" + "qq")
+VERIFY_PACK = struct.Struct("=qqqi4x" + "q2q" * 2 + "qq" * 2 + "qqqq")
 assert [x.size for x in (PAGES_PACK, APPEND_PACK, READ_PACK, ATTEND_PACK, VERIFY_PACK)] == [
     ctypes.sizeof(x) for x in (FpaPages, FpaAppendArgs, FpaReadArgs, FpaAttendArgs, FpaVerifyArgs)]
 
@@ -156,7 +157,9 @@ def lib():
         getattr(L, name).restype = ctypes.c_int
         getattr(L, name).argtypes = [ctypes.POINTER(args), _vp]
     L.fpa_attend_workspace_bytes.restype = _i64
-    L.fpa_attend_workspace_bytes.argtypes = [_i64] * 6
+    L.fpa_attend_workspace_bytes.argtypes = [_i64] * 6 + [ctypes.c_int32]
+    L.fpa_verify_workspace_bytes.restype = _i64
+    L.fpa_verify_workspace_bytes.argtypes = [_i64] * 2
     if L.fpa_abi_version() != ABI_VERSION:
         raise RuntimeError(f"libfpa.so ABI {L.fpa_abi_version()} != {ABI_VERSION}: rebuild it")
     L.fpa_source_hash.restype = ctypes.c_char_p

@@ -5,7 +5,7 @@ import functools
 import torch
 
 from . import _lib
-from ._hip import _rows_ok, device_guard, workspace
+from ._hip import _rows_ok, counters, device_guard, workspace
 
 _CODES = {torch.float16: _lib.FPA_F16, torch.float32: _lib.FPA_F32, torch.float8_e4m3fn: _lib.FPA_E4M3}
 
@@ -58,8 +58,8 @@ def read(c, table, start, n, counts, dtype):
 
 
 @functools.lru_cache(maxsize=256)
-def _attend_ws_bytes(B, H, N, D, P, prefix_length):
-    return _lib.lib().fpa_attend_workspace_bytes(B, H, N, D, P, prefix_length)
+def _attend_ws_bytes(B, H, N, D, P, prefix_length, dtype):
+    return _lib.lib().fpa_attend_workspace_bytes(B, H, N, D, P, prefix_length, dtype)
 
 
 def attend(q, c, beta, table, lengths, prefix, prefix_length):
@@ -70,13 +70,19 @@ def attend(q, c, beta, table, lengths, prefix, prefix_length):
     P = table.shape[1]
     with device_guard(dev):
         o = torch.empty((B, N, H, D), dtype=q.dtype, device=dev).transpose(1, 2)
-        nws = _attend_ws_bytes(B, H, N, D, P, prefix_length)
+        nws = _attend_ws_bytes(B, H, N, D, P, prefix_length, _CODES[q.dtype])
         ws = workspace(dev, nws) if nws else None
         a = _lib.FpaAttendArgs.from_buffer_copy(_lib.ATTEND_PACK.pack(
             _pages(c), B, N, P, _CODES[q.dtype], q.data_ptr(), *q.stride(), o.data_ptr(), *o.stride(), beta.data_ptr(),
-            table.data_ptr(), table.stride(0), lengths.data_ptr(), _ptr(prefix), prefix_length, _ptr(ws)))
+            table.data_ptr(), table.stride(0), lengths.data_ptr(), _ptr(prefix), prefix_length, _ptr(ws),
+            counters(dev, B * H).data_ptr()))
         _lib.check(_lib.lib().fpa_attend(a, _lib.stream_of(dev)))
     return o
+
+
+@functools.lru_cache(maxsize=256)
+def _verify_ws_bytes(B, V):
+    return _lib.lib().fpa_verify_workspace_bytes(B, V)
 
 
 def verify(target, draft, tokens, accept_u, sample_u):
@@ -86,9 +92,11 @@ def verify(target, draft, tokens, accept_u, sample_u):
     with device_guard(dev):
         out = torch.empty(B * (N + 2), dtype=torch.int64, device=dev)  # both results in one allocation
         accepted, out = out[:B], out[B:].view(B, N + 1)
+        ws = workspace(dev, _verify_ws_bytes(B, V))
         a = _lib.FpaVerifyArgs.from_buffer_copy(_lib.VERIFY_PACK.pack(
             B, N, V, _CODES[target.dtype], target.data_ptr(), *target.stride()[:2],
             _ptr(draft), *(draft.stride()[:2] if draft is not None else (0, 0)), tokens.data_ptr(), tokens.stride(0),
-            accept_u.data_ptr(), accept_u.stride(0), sample_u.data_ptr(), accepted.data_ptr(), out.data_ptr()))
+            accept_u.data_ptr(), accept_u.stride(0), sample_u.data_ptr(), accepted.data_ptr(), out.data_ptr(),
+            ws.data_ptr()))
         _lib.check(_lib.lib().fpa_verify(a, _lib.stream_of(dev)))
     return accepted, out

@@ -264,8 +264,11 @@ typedef struct {
     const int32_t *prefix;                 /* or NULL */
     int64_t prefix_length;
     void *workspace;                       /* fpa_attend_workspace_bytes(), 256-byte aligned */
+    int32_t *counts;                       /* B * H ints of device memory, zero before the first call; every call
+                                              leaves them zero.  Calls that may overlap need counts of their own,
+                                              as they need workspaces of their own. */
 } FpaAttendArgs;
-int64_t fpa_attend_workspace_bytes(int64_t B, int64_t H, int64_t N, int64_t D, int64_t P, int64_t prefix_length);
+int64_t fpa_attend_workspace_bytes(int64_t B, int64_t H, int64_t N, int64_t D, int64_t P, int64_t prefix_length, int32_t dtype);
 int fpa_attend(const FpaAttendArgs *args, void *stream);
 
 /* Verifies N drafted tokens of B sequences.  target: probabilities (B, N + 1, V), draft: (B, N, V) or NULL for
@@ -285,7 +288,9 @@ typedef struct {
     const float *sample_u;                 /* (B,), in [0, 1) */
     int64_t *accepted;
     int64_t *out;                          /* contiguous */
+    void *workspace;                       /* fpa_verify_workspace_bytes(), 256-byte aligned */
 } FpaVerifyArgs;
+int64_t fpa_verify_workspace_bytes(int64_t B, int64_t V);
 int fpa_verify(const FpaVerifyArgs *args, void *stream);
 
 /* Message of the last failed call on this host thread ("" if none). */
