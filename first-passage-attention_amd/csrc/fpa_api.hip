@@ -444,13 +444,22 @@ Pages pages_of(const FpaPages &c) {
 // Parts of the sequences' own pages and of the prefix, and their scratch.
 struct AttendPlan {
     int chunk, nchunk, pchunk = 1, npchunk = 0;
+    bool alone;
     int64_t ml, total;  // float offset of the statistics, bytes
 };
-AttendPlan attend_plan(int64_t B, int64_t H, int64_t N, int64_t D, int64_t P, int64_t PL, int32_t dtype) {
+AttendPlan attend_plan(int64_t B, int64_t H, int64_t N, int64_t D, int64_t P, int64_t PL, int32_t dtype, int32_t store) {
     AttendPlan a;
     const int64_t rows = attend_rows(B * N, (int)D, dtype);
-    attend_parts(B * H * ((N + 15) / 16), P, (int)D, a.chunk, a.nchunk);
-    if (PL > 0) attend_parts(H * ((B * N + rows - 1) / rows), (PL + PG - 1) / PG, (int)D, a.pchunk, a.npchunk);
+    const int64_t items = B * H * ((N + 15) / 16);
+    a.alone = attend_alone(B, H, N, P, (int)D, dtype, PL > 0);
+    if (a.alone) {
+        a.chunk = (int)P;
+        a.nchunk = 1;
+    } else {
+        attend_parts(items, P, (int)D, attend_steps((int)D, dtype, store, N, PL > 0, 0), 0, a.chunk, a.nchunk);
+    }
+    if (PL > 0) attend_parts(H * ((B * N + rows - 1) / rows), (PL + PG - 1) / PG, (int)D, attend_steps((int)D, dtype, store, N, true, (int)rows / 16),
+                             a.alone ? (B * H + attend_waves((int)D) - 1) / attend_waves((int)D) : items * a.nchunk, a.pchunk, a.npchunk);
     const int64_t slots = (a.nchunk <= 1 && a.npchunk == 0) ? 0 : (int64_t)(a.nchunk + a.npchunk) * B * H * N;
     a.ml = align64(slots * D);
     a.total = (a.ml + align64(slots * 2)) * (int64_t)sizeof(float);
@@ -498,9 +507,15 @@ int fpa_cache_read(const FpaReadArgs *a, void *stream) {
     return e != hipSuccess ? hip_fail(e, "fpa_cache_read launch") : FPA_OK;
 }
 
-int64_t fpa_attend_workspace_bytes(int64_t B, int64_t H, int64_t N, int64_t D, int64_t P, int64_t prefix_length, int32_t dtype) {
+int64_t fpa_attend_workspace_bytes(int64_t B, int64_t H, int64_t N, int64_t D, int64_t P, int64_t prefix_length, int32_t dtype, int32_t store) {
     if (B < 1 || H < 1 || N < 1 || D < 1 || P < 1) return 0;
-    return attend_plan(B, H, N, D, P, prefix_length, dtype).total;
+    return attend_plan(B, H, N, D, P, prefix_length, dtype, store).total;
+}
+
+int64_t fpa_attend_counts(int64_t B, int64_t H, int64_t N) {
+    if (B < 1 || H < 1 || N < 1) return 0;
+    const int64_t tiles = (B * N + 15) / 16;
+    return H * (B > tiles ? B : tiles);
 }
 
 int fpa_attend(const FpaAttendArgs *a, void *stream) {
@@ -515,7 +530,7 @@ int fpa_attend(const FpaAttendArgs *a, void *stream) {
         return fail(FPA_ERR_INVALID, "prefix_length must be between 0 and " + std::to_string((int64_t)MAX_NB * G));
     if (a->prefix_length > 0 && !a->prefix) return fail(FPA_ERR_INVALID, "prefix is NULL");
     const int64_t H = a->cache.H, D = a->cache.D;
-    const AttendPlan pl = attend_plan(a->B, H, a->N, D, a->P, a->prefix_length, a->dtype);
+    const AttendPlan pl = attend_plan(a->B, H, a->N, D, a->P, a->prefix_length, a->dtype, a->cache.store);
     if (pl.total > 0 && (a->workspace == nullptr || (reinterpret_cast<uintptr_t>(a->workspace) & 255) != 0))
         return fail(FPA_ERR_INVALID, "workspace must be non-NULL and 256-byte aligned");
     if (!a->counts || (reinterpret_cast<uintptr_t>(a->counts) & 3) != 0) return fail(FPA_ERR_INVALID, "counts must be non-NULL");
@@ -532,7 +547,7 @@ int fpa_attend(const FpaAttendArgs *a, void *stream) {
     p.ml = p.part + pl.ml;
     p.counts = a->counts;
     p.B = (int)a->B; p.N = (int)a->N; p.P = (int)a->P; p.PL = (int)a->prefix_length;
-    p.chunk = pl.chunk; p.nchunk = pl.nchunk; p.pchunk = pl.pchunk; p.npchunk = pl.npchunk;
+    p.chunk = pl.chunk; p.nchunk = pl.nchunk; p.pchunk = pl.pchunk; p.npchunk = pl.npchunk; p.alone = pl.alone;
     p.sc2 = LOG2E / sqrtf((float)D);
     const hipError_t e = launch_attend(p, a->dtype, a->cache.store, (int)D, reinterpret_cast<hipStream_t>(stream));
     return e != hipSuccess ? hip_fail(e, "fpa_attend launch") : FPA_OK;

@@ -1,1088 +1,59 @@
-// fpa_attend.hip -- First Passage Attention of new tokens against a paged cache.
-//
-// Query i of N stands at position t = len - N + i of its sequence and attends to the keys s <= t:
-//   o_t = sum_s softmax_s(q_t . k_s / sqrt(D) + beta min(0, X_ts - psi_s)) v_s,   X_ts = min_{s < u <= t} phi_u
-// (X_tt is +inf).  A shared prefix of PL positions comes before the sequence's own position 0: for its keys
-//   X_ts = min(min_{s < u < PL} phi_u, min_{0 <= u <= t} phi_u of the sequence itself),
-// so that only the second term differs between the requests, and the rows of all of them form one product
-// with the prefix's K and V.
-//
-// A wave takes a page (64 keys) at a time, from the last to the first, and carries the running minimum of phi along;
-// what lies between its pages and its queries is one phi_min value a page.  Both cache operands go from HBM straight
-// into the registers of the 16x16 MFMA: the pages hold K by rows and V transposed, so that an operand of either
-// product is a run of consecutive values.  The next page's K is loaded as soon as this one's scores are formed, the
-// next V when this one's is used up.
-//
-// Two forms of the page step:
-//   wide  16 rows in the columns of S^T = K Q^T, O^T += V^T P^T (N > 4, and the prefix, there 32 rows with every K and
-//         V operand used twice).  The key of score register (a, j) of lane group g is 16 g + 4 a + j, so that a
-//         lane's 16 weights belong to 16 consecutive keys: as they stand they are the operand of the second product, whose
-//         other operand is 16 consecutive values of a V^T row, and the range minimum is a scan inside the lane.
-//   few   up to 4 rows, S = Q K^T with the queries repeated over the 16 rows, so that lane l finds the scores of one key,
-//         63 - l.  Masks, exponentials and scales then cost one operation a page and row where the wide form spends 16
-//         on columns that hold no query; the range minimum is a scan over the lanes, and the weights go through
-//         64 values of LDS into the operand of O = P V.
-//
-// A sequence, and the prefix, is cut into parts of whole pages that run side by side, each wave of a workgroup taking a
-// quarter of its part.  Partial results (O, maximum, sum) go to the workspace, and the workgroup that finishes a sequence's
-// last part joins them, in the parts' order whoever that is: no second kernel, the same bits every time.  With a prefix
-// a second kernel joins them.
-//
-// Softmax statistics and O are fp32.  P is rounded to fp16 for fp16 queries; the running maximum is raised only where a
-// weight would pass 2^8, which costs fp16 nothing (what it loses lies 2^-25 below 1) and saves most rescalings; fp32
-// queries keep fp32 throughout.  With e4m3 pages the row's power of two of V goes into the logit: the weights
-// w_s = p_s 2^e_s are what multiplies the codes, the running maximum is that of w, so that w fills fp16's range whatever
-// the scales are, and the sum takes w_s 2^-e_s.
-//
-// What a query must not see is never multiplied: masked scores are replaced, V rows behind the sequence's end
-// are cleared, and an infinity or NaN in a V row that only some of the rows see is left out of the product and
-// added for those alone.
-#include <type_traits>
-
-#include "fpa_common.h"
-#include "fpa_serve.h"
+// fpa_attend.hip -- how the attention against a cache is cut into parts, and its dispatch over types; the kernels are in
+// fpa_attend.h, built by the fpa_attend_*.hip files.
+#include "fpa_attend.h"
 
 namespace fpa {
 
-namespace {
-
-constexpr int CW = 16;  // query rows of a wave
-
-__device__ __forceinline__ int uni(int x) { return __builtin_amdgcn_readfirstlane(x); }
-__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
-
-// N consecutive cache values of a lane, first as loaded, then as matrix operands.
-template <typename TS, int N> struct Raw {
-    static constexpr int BYTES = N * (int)sizeof(TS);
-    static_assert(BYTES % 4 == 0, "whole words");
-    uint32_t w[BYTES / 4];
-    __device__ __forceinline__ void load(const TS *p) {
-        const char *b = reinterpret_cast<const char *>(p);
-        if constexpr (BYTES % 16 == 0) {
-#pragma unroll
-            for (int i = 0; i < BYTES / 16; ++i) {
-                const u32x4 x = *reinterpret_cast<const u32x4 *>(b + 16 * i);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) w[4 * i + j] = x[j];
-            }
-        } else if constexpr (BYTES == 8) {
-            const uint2 x = *reinterpret_cast<const uint2 *>(b);
-            w[0] = x.x;
-            w[1] = x.y;
-        } else {
-            static_assert(BYTES == 4, "4, 8 or a multiple of 16 bytes");
-            w[0] = *reinterpret_cast<const uint32_t *>(b);
-        }
-    }
-    // values 4 i .. 4 i + 3
-    __device__ __forceinline__ h4 half4(int i) const {
-        if constexpr (sizeof(TS) == 2) {
-            const uint2 x = make_uint2(w[2 * i], w[2 * i + 1]);
-            return __builtin_bit_cast(h4, x);
-        } else {
-            static_assert(sizeof(TS) == 1, "fp16 operands come from fp16 or e4m3");
-            const h2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w[i], 1.0f, false);
-            const h2 b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w[i], 1.0f, true);
-            return h4{a[0], a[1], b[0], b[1]};
-        }
-    }
-    __device__ __forceinline__ f32x4 float4_(int i) const {
-        if constexpr (sizeof(TS) == 4) {
-            return f32x4{__uint_as_float(w[4 * i]), __uint_as_float(w[4 * i + 1]), __uint_as_float(w[4 * i + 2]),
-                         __uint_as_float(w[4 * i + 3])};
-        } else {
-            static_assert(sizeof(TS) == 1, "fp32 operands come from fp32 or e4m3");
-            const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[i], false);
-            const f32x2 b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[i], true);
-            return f32x4{a[0], a[1], b[0], b[1]};
-        }
-    }
-};
-
-// Matrix operands of N consecutive values per lane: fp16 as h4 quads, fp32 as f32x4 quads.
-template <typename TQ> struct Quad;
-template <> struct Quad<f16> {
-    typedef h4 t;
-};
-template <> struct Quad<float> {
-    typedef f32x4 t;
-};
-template <typename TQ, typename TS, int N> __device__ __forceinline__ typename Quad<TQ>::t quad(const Raw<TS, N> &r, int i) {
-    if constexpr (sizeof(TQ) == 2)
-        return r.half4(i);
-    else
-        return r.float4_(i);
-}
-// Infinities and NaN are told by the stored bits, as integers: this file is compiled without NaN in mind.
-template <typename TS> __device__ __forceinline__ bool beyond_bits(uint32_t bits) {  // of one stored value
-    if constexpr (sizeof(TS) == 1) return (bits & 0x7fu) == 0x7fu;
-    if constexpr (sizeof(TS) == 2) return (bits & 0x7c00u) == 0x7c00u;
-    return (bits & 0x7f800000u) == 0x7f800000u;
-}
-// Clears the values of a run from element `n` on and (unless KEEP) those that are not finite; true if there were
-// such before n.
-template <bool KEEP, typename TS, int N> __device__ __forceinline__ bool clean(Raw<TS, N> &r, int n) {
-    constexpr int PW = 4 / sizeof(TS), BITS = 8 * sizeof(TS);  // values of a word
-    constexpr uint32_t ONE = BITS == 32 ? 0xffffffffu : (1u << (BITS % 32)) - 1;
-    bool some = false;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const int sh = i % PW * BITS;
-        const bool off = !KEEP && beyond_bits<TS>(r.w[i / PW] >> sh & ONE);
-        if (i >= n || off) r.w[i / PW] &= ~(ONE << sh);
-        some |= i < n && off;
-    }
-    return some;
-}
-
-constexpr uint32_t BAD = 0xbf800000u;  // -1.0f in place of a row's sum: its table names no page, or its length passes the table
-// NaN that the compiler does not see as one (it may drop what it can tell to be NaN).
-__device__ __forceinline__ float quiet_nan() {
-    uint32_t b = 0x7fc00000u;
-    asm("" : "+v"(b));
-    return __uint_as_float(b);
-}
-
-// The infinity or NaN at vx, or 0 for a finite value.
-template <typename TS> __device__ __forceinline__ float not_finite(const TS *vx) {
-    if constexpr (sizeof(TS) == 1)
-        return beyond_bits<TS>(vx->code) ? quiet_nan() : 0.f;
-    else if constexpr (sizeof(TS) == 2)
-        return beyond_bits<TS>(*reinterpret_cast<const uint16_t *>(vx)) ? (float)*vx : 0.f;
-    else
-        return beyond_bits<TS>(*reinterpret_cast<const uint32_t *>(vx)) ? *vx : 0.f;
-}
-
-// acc += A B^T over NQ quads of the contraction (A: row lane % 16, B: column lane % 16, both of the lane
-// group's consecutive values).
-template <int NQ> __device__ __forceinline__ f32x4 mma(const h4 (&a)[NQ], const h4 (&b)[NQ], f32x4 acc) {
-    if constexpr (NQ == 1) {
-        return __builtin_amdgcn_mfma_f32_16x16x16f16(a[0], b[0], acc, 0, 0, 0);
-    } else {
-#pragma unroll
-        for (int i = 0; i < NQ; i += 2)
-            acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_shufflevector(a[i], a[i + 1], 0, 1, 2, 3, 4, 5, 6, 7),
-                                                         __builtin_shufflevector(b[i], b[i + 1], 0, 1, 2, 3, 4, 5, 6, 7),
-                                                         acc, 0, 0, 0);
-        return acc;
-    }
-}
-template <int NQ> __device__ __forceinline__ f32x4 mma(const f32x4 (&a)[NQ], const f32x4 (&b)[NQ], f32x4 acc) {
-#pragma unroll
-    for (int i = 0; i < NQ; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i][e], b[i][e], acc, 0, 0, 0);
-    return acc;
-}
-
-__device__ __forceinline__ float min_groups(float x) {
-    x = fminf(x, __shfl_xor(x, 16, 64));
-    return fminf(x, __shfl_xor(x, 32, 64));
-}
-__device__ __forceinline__ float max_groups(float x) {
-    x = fmaxf(x, __shfl_xor(x, 16, 64));
-    return fmaxf(x, __shfl_xor(x, 32, 64));
-}
-__device__ __forceinline__ float sum_groups(float x) {
-    x += __shfl_xor(x, 16, 64);
-    return x + __shfl_xor(x, 32, 64);
-}
-
-// Length of sequence b, at most what its table holds.
-__device__ __forceinline__ int seq_len(const AttendParams &p, int b, bool &bad) {
-    const int L = p.lengths[b];
-    const int64_t cap = (int64_t)p.P * PG;
-    if (L > cap) bad = true;
-    return L < 0 ? 0 : (L > cap ? (int)cap : L);
-}
-
-// LDS written by the wave's other lanes is read after this (one wave's LDS accesses are in order; the compiler keeps them so).
-__device__ __forceinline__ void wave_sync() {
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
-
-// Inclusive minimum over the lanes 0 .. l.
-template <int CTRL, int ROWS> __device__ __forceinline__ float dpp_or_inf(float x) {
-    return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0x7f800000, (int)__float_as_uint(x), CTRL, ROWS, 0xf, false));
-}
-__device__ __forceinline__ float scan_min(float x) {
-    x = fminf(x, dpp_or_inf<0x111, 0xf>(x));  // within rows of 16: 1, 2, 4, 8 lanes down
-    x = fminf(x, dpp_or_inf<0x112, 0xf>(x));
-    x = fminf(x, dpp_or_inf<0x114, 0xf>(x));
-    x = fminf(x, dpp_or_inf<0x118, 0xf>(x));
-    x = fminf(x, dpp_or_inf<0x142, 0xa>(x));  // lane 15 into row 1, 47 into row 3
-    return fminf(x, dpp_or_inf<0x143, 0xc>(x));  // lane 31 into rows 2 and 3
-}
-__device__ __forceinline__ float one_lane_down(float x) { return dpp_or_inf<0x138, 0xf>(x); }  // +inf in lane 0
-__device__ __forceinline__ float lane_value(float x, int l) { return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(x), l)); }
-template <int CTRL, int ROWS> __device__ __forceinline__ float dpp_self(float x) {
-    return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp((int)__float_as_uint(x), (int)__float_as_uint(x), CTRL, ROWS, 0xf, false));
-}
-__device__ __forceinline__ float wave_max(float x) {
-    x = fmaxf(x, dpp_self<0x111, 0xf>(x));
-    x = fmaxf(x, dpp_self<0x112, 0xf>(x));
-    x = fmaxf(x, dpp_self<0x114, 0xf>(x));
-    x = fmaxf(x, dpp_self<0x118, 0xf>(x));
-    x = fmaxf(x, dpp_self<0x142, 0xa>(x));
-    x = fmaxf(x, dpp_self<0x143, 0xc>(x));
-    return lane_value(x, 63);
-}
-__device__ __forceinline__ float wave_min(float x) { return lane_value(scan_min(x), 63); }
-
-constexpr float SLACK = 8.f;  // a weight may reach 2^SLACK before the running maximum is raised
-
-// Values that another workgroup of this launch reads: agent-scope accesses, which go past the caches that the
-// XCDs do not share.
-__device__ __forceinline__ void put2(float *p, float a, float b) {
-    const uint64_t v = (uint64_t)__float_as_uint(b) << 32 | __float_as_uint(a);
-    __hip_atomic_store(reinterpret_cast<uint64_t *>(p), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ __forceinline__ f32x2 get2(const float *p) {
-    const uint64_t v = __hip_atomic_load(reinterpret_cast<const uint64_t *>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    return f32x2{__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32))};
-}
-
-__device__ __forceinline__ float exp_or_0(float m, float ref) { return fexp2(m - (ref == ninf() ? 0.f : ref)); }
-
-// Rows of a prefix tile.
-template <int NC> constexpr int tile_rows() { return CW * NC; }
-
-// Waves of a workgroup: as many as two a SIMD (their registers end at 256), so that most sequences need no second part.
-constexpr int waves(int D) { return D <= 128 ? 8 : 4; }
-
-// Parts of a sequence's own pages: one at least, which may be empty.
-__device__ __forceinline__ int own_parts(const AttendParams &p, int L) {
-    const int n = ((L + PG - 1) / PG + p.chunk - 1) / p.chunk;
-    return n < 1 ? 1 : n;
-}
-
-// LDS of a workgroup.
-template <int D, int NC> struct Shared {
-    static constexpr int NW = waves(D);
-    float fold[NW / 2][NC * CW * D];  // accumulators on their way to another wave
-    float stat[NW / 2][NC * CW * 2];
-    float behind[NW];
-    int done;
-    float join[64 * NW][6];
-};
-
-// Adds up the parts of the N rows of sequence b, head h, in order, and writes the output rows; NT threads.
-template <typename TQ, int D, int NT> __device__ void join_parts(const AttendParams &p, int b, int h, float (*join)[6]) {
-    const int tid = thread_x(), H = p.c.H;
-    bool lost = false;
-    const int L = seq_len(p, b, lost);
-    const int own = own_parts(p, L), parts = own + p.npchunk;
-    const int64_t R = (int64_t)p.B * H * p.N, row0 = ((int64_t)b * H + h) * p.N;
-    const int E = p.N * (D / 4);                           // quads of the output
-    const int sets = E < NT ? NT / E : 1;                // threads that share a quad's parts
-    for (int e0 = 0; e0 < E; e0 += NT) {
-        const int e = e0 + tid % min(E, NT), set = E < NT ? tid / E : 0;
-        float m = ninf(), l = 0.f;
-        f32x4 x = {0.f, 0.f, 0.f, 0.f};
-        bool bad = lost;
-        if (e < E && set < sets) {
-            const int r = e / (D / 4), d = e % (D / 4) * 4;
-            constexpr int AT_ONCE = 4;  // parts whose loads are in flight together
-            for (int k0 = set; k0 < parts; k0 += AT_ONCE * sets) {
-                f32x2 s[AT_ONCE], u[AT_ONCE], v[AT_ONCE];
-#pragma unroll
-                for (int j = 0; j < AT_ONCE; ++j) {
-                    const int k = min(k0 + j * sets, parts - 1);
-                    const int64_t slot = (int64_t)(k < own ? k : p.nchunk + k - own) * R + row0 + r;
-                    s[j] = get2(p.ml + 2 * slot);
-                    u[j] = get2(p.part + slot * D + d);
-                    v[j] = get2(p.part + slot * D + d + 2);
-                }
-#pragma unroll
-                for (int j = 0; j < AT_ONCE; ++j) {
-                    if (k0 + j * sets >= parts) break;
-                    bad |= __float_as_uint(s[j][1]) == BAD;
-                    const float mn = fmaxf(m, s[j][0]), a = exp_or_0(m, mn), w = exp_or_0(s[j][0], mn);
-                    l = l * a + s[j][1] * w;
-                    x[0] = x[0] * a + u[j][0] * w;
-                    x[1] = x[1] * a + u[j][1] * w;
-                    x[2] = x[2] * a + v[j][0] * w;
-                    x[3] = x[3] * a + v[j][1] * w;
-                    m = mn;
-                }
-            }
-        }
-        if (sets > 1) {
-            __syncthreads();
-            join[tid][0] = m;
-            join[tid][1] = bad ? __uint_as_float(BAD) : l;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) join[tid][2 + j] = x[j];
-            __syncthreads();
-            if (set == 0)
-                for (int k = 1; k < sets; ++k) {
-                    const float *o = join[k * E + tid];
-                    bad |= __float_as_uint(o[1]) == BAD;
-                    const float mn = fmaxf(m, o[0]), a = exp_or_0(m, mn), w = exp_or_0(o[0], mn);
-                    l = l * a + o[1] * w;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) x[j] = x[j] * a + o[2 + j] * w;
-                    m = mn;
-                }
-        }
-        if (e < E && set == 0) {
-            const int r = e / (D / 4), d = e % (D / 4) * 4;
-            const bool none = (__float_as_uint(l) << 1) == 0;
-            TQ *o = static_cast<TQ *>(p.o) + (int64_t)b * p.so.b + (int64_t)h * p.so.h + (int64_t)r * p.so.t + d;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) o[j] = (TQ)(bad ? quiet_nan() : none ? 0.f : x[j] / l);
-        }
-    }
-}
-
-// Four neighbouring features of one row's result: the output itself if this part is all of it, else the part's.
-template <typename TQ, int D>
-__device__ __forceinline__ void put_row(const AttendParams &p, bool whole, int slot, int b, int h, int i, int d, f32x4 x, float m, float l) {
-    const bool bad = __float_as_uint(l) == BAD;
-    if (whole) {
-        const bool none = (__float_as_uint(l) << 1) == 0;
-        TQ *o = static_cast<TQ *>(p.o) + (int64_t)b * p.so.b + (int64_t)h * p.so.h + (int64_t)i * p.so.t + d;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) o[j] = (TQ)(bad ? quiet_nan() : none ? 0.f : x[j] / l);
-    } else {
-        const int64_t at = (int64_t)slot * p.B * p.c.H * p.N + ((int64_t)b * p.c.H + h) * p.N + i;
-        put2(p.part + at * D + d, x[0], x[1]);
-        put2(p.part + at * D + d + 2, x[2], x[3]);
-        if (d == 0) put2(p.ml + 2 * at, m, l);
-    }
-}
-
-// Counts this workgroup's part of sequence b (one thread): true if it is the last, which leaves the count at 0
-// for the next launch.  Its stores are complete: the wave that made them has waited for them.
-__device__ __forceinline__ int last_part(const AttendParams &p, int b, int h) {
-    bool lost = false;
-    const int all = own_parts(p, seq_len(p, b, lost)) * ((p.N + CW - 1) / CW);
-    int32_t *count = p.counts + (int64_t)b * p.c.H + h;
-    const int before = __hip_atomic_fetch_add(count, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    if (before + 1 < all) return 0;
-    __hip_atomic_store(count, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    return 1;
-}
-__device__ __forceinline__ void stores_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
-
-// The page numbers of a wave's pages [ws, we) (at most 64), one a lane; pages that do not exist become 0 and are told.
-__device__ __forceinline__ int page_numbers(const AttendParams &p, const int32_t *table, int ws, int we, int lane, bool &missing) {
-    int page = 0;
-    if (ws + lane < we) {
-        page = table[ws + lane];
-        if ((uint32_t)page >= (uint64_t)p.c.n) {
-            missing = true;
-            page = 0;
-        }
-    }
-    return page;
-}
-// min of phi_min over the pages k0, k0 + step, .. < k1 of this lane.
-__device__ __forceinline__ float lane_min(const AttendParams &p, const int32_t *table, int h, int k0, int k1, int step, bool &missing) {
-    float m = pinf();
-#pragma unroll 4
-    for (int k = k0; k < k1; k += step) {
-        const int page = table[k];
-        const bool there = (uint32_t)page < (uint64_t)p.c.n;
-        missing |= !there;
-        const float x = p.c.phi_min[(int64_t)(there ? page : 0) * p.c.H + h];
-        m = there ? fminf(m, x) : m;
-    }
-    return m;
-}
-
-// ---------------------------------------------------------------------------
-// few
-// ---------------------------------------------------------------------------
-template <typename TQ, typename TS, int D, int NR, typename SH>
-__device__ __forceinline__ void few_rows(const AttendParams &p, int b, int h, int part, SH &sh, TQ (*weights)[NR * PG]) {
-    typedef typename Quad<TQ>::t quad_t;
-    constexpr int DG = D / 4, ND = D / 16, NW = waves(D);
-    // The next page's operands in registers while this page is worked on, where 64 rows of K and of V leave room for it.
-    constexpr bool HOLD = D * sizeof(TS) <= 256;
-    const int tid = thread_x(), lane = tid % 64, wave = uni(tid / 64), c = lane % 16, g = lane / 16;
-    const int H = p.c.H;
-    bool missing = false;
-    const int L = uni(seq_len(p, b, missing));
-    const int npg = (L + PG - 1) / PG;
-    const int ps = part * p.chunk, pe = min(ps + p.chunk, npg);
-    const int32_t *table = p.table + (int64_t)b * p.stable;
-    const int t0 = L - p.N;                      // position of row 0
-    const int pf = t0 >= 0 ? (t0 + 1) / PG : 0;  // pages that every row sees whole
-    const int per = pe > ps ? (pe - ps + NW - 1) / NW : 0;
-    const int ws = ps + wave * per, we = min(ws + per, pe);
-    // Everything that names a page first, then what those name: two trips to memory before the first scores.
-    const int pages = page_numbers(p, table, ws, we, lane, missing);
-    const bool far = pf > ps + PG;  // more whole pages behind than one load of the wave covers
-    const int behind_page = page_numbers(p, table, we, ws < we ? (far ? min(pe, pf) : pf) : 0, lane, missing);
-    const int part_page = page_numbers(p, table, max(we, pf), ws < we ? npg : 0, lane, missing);  // at most two
-    float mine = we + lane < (far ? min(pe, pf) : pf) && ws < we ? p.c.phi_min[(int64_t)behind_page * H + h] : pinf();
-    auto head_page = [&](int pg) { return (int64_t)__builtin_amdgcn_readlane(pages, pg - ws) * H + h; };
-
-    const int key = 63 - lane;
-    Raw<TS, DG> kr[4];
-    Raw<TS, 16> vr[ND];
-    float phv = 0.f, psv = 0.f;
-    int ke = 0, ve = 0;
-    auto load_k = [&](int64_t ph) __attribute__((always_inline)) {
-        const TS *kp = static_cast<const TS *>(p.c.k) + ph * PG * D;
-        if constexpr (HOLD) {
-#pragma unroll
-            for (int a = 0; a < 4; ++a) kr[a].load(kp + (63 - 16 * a - c) * D + g * DG);
-        }
-        phv = p.c.phi[ph * PG + key];
-        psv = p.c.psi[ph * PG + key];
-        if constexpr (sizeof(TS) == 1) ke = p.c.k_exp[ph * PG + key];
-    };
-    auto load_v = [&](int64_t ph) __attribute__((always_inline)) {
-        const TS *vp = static_cast<const TS *>(p.c.v) + ph * PG * D;
-        if constexpr (sizeof(TS) == 1) ve = p.c.v_exp[ph * PG + key];
-        if constexpr (HOLD) {
-#pragma unroll
-            for (int d = 0; d < ND; ++d) vr[d].load(vp + (16 * d + c) * PG + 16 * g);
-        }
-    };
-    if (ws < we) {
-        const int64_t ph = head_page(we - 1);
-        load_k(ph);
-        load_v(ph);
-    }
-
-    quad_t qv[DG / 4];
-    {
-        const int i = NR == 1 ? 0 : c % NR;
-        Raw<TQ, DG> r;
-        r.load(static_cast<const TQ *>(p.q) + (int64_t)b * p.sq.b + (int64_t)h * p.sq.h + (int64_t)min(i, p.N - 1) * p.sq.t + g * DG);
-#pragma unroll
-        for (int k = 0; k < DG / 4; ++k) qv[k] = quad<TQ>(r, k);  // rows past N repeat the last: never written
-    }
-    const float beta2 = p.beta[h] * LOG2E;
-
-    // min of phi from the wave's pages on: whole pages, those beyond 64 by all waves together, then the at most two
-    // pages that some rows see in part
-    float carry[NR];
-    {
-        mine = wave_min(mine);
-        if (far) {
-            const float m = wave_min(lane_min(p, table, h, pe + tid, pf, 64 * NW, missing));
-            if (lane == 0) sh.behind[wave] = m;
-            __syncthreads();
-#pragma unroll
-            for (int w = 0; w < NW; ++w) mine = fminf(mine, sh.behind[w]);
-        }
-#pragma unroll
-        for (int j = 0; j < NR; ++j) carry[j] = mine;
-        if (ws < we) {
-            for (int k = max(we, pf); k < npg; ++k) {
-                const int64_t ph = (int64_t)__builtin_amdgcn_readlane(part_page, k - max(we, pf)) * H + h;
-                const float f = p.c.phi[ph * PG + lane];
-#pragma unroll
-                for (int j = 0; j < NR; ++j) carry[j] = fminf(carry[j], wave_min(k * PG + lane <= min(t0 + j, L - 1) ? f : pinf()));
-            }
-        }
-    }
-
-    f32x4 acc[ND];
-#pragma unroll
-    for (int d = 0; d < ND; ++d) acc[d] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float m[NR], l[NR];  // the maximum is the wave's, the sum the lane's
-#pragma unroll
-    for (int j = 0; j < NR; ++j) {
-        m[j] = ninf();
-        l[j] = 0.f;
-    }
-    TQ *wl = weights[wave];
-
-    auto page_step = [&](auto tail_tag, int pg) __attribute__((always_inline)) {
-        constexpr bool TAIL = decltype(tail_tag)::value;
-        const int pos = pg * PG + key;
-        const int64_t next = pg > ws ? head_page(pg - 1) : 0;
-        const int64_t at = HOLD ? 0 : head_page(pg) * PG * D;
-        f32x4 s[4];
-#pragma unroll
-        for (int a = 0; a < 4; ++a) {
-            if constexpr (!HOLD) kr[a].load(static_cast<const TS *>(p.c.k) + at + (63 - 16 * a - c) * D + g * DG);
-            quad_t kq[DG / 4];
-#pragma unroll
-            for (int k = 0; k < DG / 4; ++k) kq[k] = quad<TQ>(kr[a], k);
-            s[a] = mma<DG / 4>(qv, kq, f32x4{0.f, 0.f, 0.f, 0.f});
-        }
-        float t[NR];
-        if constexpr (!TAIL) {
-            const float inc = scan_min(phv), x = one_lane_down(inc), all = lane_value(inc, 63);
-#pragma unroll
-            for (int j = 0; j < NR; ++j) {
-                t[j] = fminf(x, carry[j]);
-                carry[j] = fminf(carry[j], all);
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < NR; ++j) {
-                const float inc = scan_min(pos <= min(t0 + j, L - 1) ? phv : pinf());
-                t[j] = fminf(one_lane_down(inc), carry[j]);
-                carry[j] = fminf(carry[j], lane_value(inc, 63));
-            }
-        }
-        const float sc = sizeof(TS) == 1 ? p.sc2 * pow2(ke) : p.sc2;
-        bool up = false;
-#pragma unroll
-        for (int j = 0; j < NR; ++j) {
-            const float sj = g < 2 ? (g == 0 ? s[0][j] : s[1][j]) : (g == 2 ? s[2][j] : s[3][j]);
-            t[j] = (sizeof(TS) == 1 ? sj * sc + (float)ve : sj * sc) + beta2 * fminf(t[j] - psv, 0.f);
-            if (TAIL && pos > min(t0 + j, L - 1)) t[j] = ninf();
-            up |= t[j] > m[j] + SLACK;
-        }
-        if (pg > ws) load_k(next);
-        if (__any(up)) {  // rare after the first pages
-#pragma unroll
-            for (int j = 0; j < NR; ++j) {
-                const float mn = fmaxf(m[j], wave_max(t[j]));
-                const float alpha = exp_or_0(m[j], mn);
-                m[j] = mn;
-                l[j] *= alpha;
-#pragma unroll
-                for (int d = 0; d < ND; ++d) acc[d][j] *= alpha;
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < NR; ++j) {
-            const float w = exp_or_0(t[j], m[j]);
-            wl[j * PG + key] = (TQ)w;
-            t[j] = w;
-            l[j] += sizeof(TS) == 1 ? w * pow2(-ve) : w;
-        }
-        wave_sync();
-        quad_t pq[4];
-#pragma unroll
-        for (int a = 0; a < 4; ++a) pq[a] = *reinterpret_cast<const quad_t *>(wl + (NR == 1 ? 0 : c % NR) * PG + 16 * g + 4 * a);
-        wave_sync();
-        bool some = false;
-#pragma unroll
-        for (int d = 0; d < ND; ++d) {
-            if constexpr (!HOLD) vr[d].load(static_cast<const TS *>(p.c.v) + at + (16 * d + c) * PG + 16 * g);
-            if constexpr (TAIL) some |= clean<NR == 1>(vr[d], L - pg * PG - 16 * g);
-            quad_t vq[4];
-#pragma unroll
-            for (int a = 0; a < 4; ++a) vq[a] = quad<TQ>(vr[d], a);
-            acc[d] = mma<4>(pq, vq, acc[d]);
-        }
-        if (TAIL && NR > 1 && __any(some)) {  // infinities and NaN, for the rows that see them
-            const TS *vp = static_cast<const TS *>(p.c.v) + head_page(pg) * PG * D;
-            for (int e = 0; e < PG; ++e) {
-#pragma unroll
-                for (int d = 0; d < ND; ++d) {
-                    const float y = not_finite(vp + (16 * d + c) * PG + e);
-#pragma unroll
-                    for (int j = 0; j < NR; ++j) {
-                        const float w = __shfl(t[j], 63 - e, 64);
-                        if (pg * PG + e <= t0 + j && __float_as_uint(y) != 0) acc[d][j] += w * y;
-                    }
-                }
-            }
-        }
-        if (pg > ws) load_v(next);
-    };
-    int pg = we - 1;
-    for (; pg >= ws && pg >= pf; --pg) page_step(std::true_type{}, pg);
-    for (; pg >= ws; --pg) page_step(std::false_type{}, pg);
-
-    // The waves' results together, the upper half into the lower, down to wave 0.
-    const bool bad = __any(missing);
-#pragma unroll
-    for (int j = 0; j < NR; ++j) {
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) l[j] += __shfl_xor(l[j], o, 64);
-        if (bad) l[j] = __uint_as_float(BAD);
-    }
-#pragma unroll
-    for (int from = NW / 2; from >= 1; from /= 2) {
-        __syncthreads();
-        if (wave >= from && wave < 2 * from) {
-#pragma unroll
-            for (int j = 0; j < NR; ++j) {
-                if (lane == 0) {
-                    sh.stat[wave - from][2 * j] = m[j];
-                    sh.stat[wave - from][2 * j + 1] = l[j];
-                }
-#pragma unroll
-                for (int d = 0; d < ND; ++d)
-                    if (g == d % 4) sh.fold[wave - from][j * D + 16 * d + c] = acc[d][j];
-            }
-        }
-        __syncthreads();
-        if (wave < from) {
-#pragma unroll
-            for (int j = 0; j < NR; ++j) {
-                const float m2 = sh.stat[wave][2 * j], l2 = sh.stat[wave][2 * j + 1], mn = fmaxf(m[j], m2);
-                const float a = exp_or_0(m[j], mn), w = exp_or_0(m2, mn);
-                const bool lost = __float_as_uint(l[j]) == BAD || __float_as_uint(l2) == BAD;
-                m[j] = mn;
-                l[j] = lost ? __uint_as_float(BAD) : l[j] * a + l2 * w;
-#pragma unroll
-                for (int d = 0; d < ND; ++d) acc[d][j] = acc[d][j] * a + sh.fold[wave][j * D + 16 * d + c] * w;
-            }
-        }
-    }
-    const bool whole = p.npchunk == 0 && own_parts(p, L) == 1;
-    if (wave == 0) {
-#pragma unroll
-        for (int j = 0; j < NR; ++j)
-#pragma unroll
-            for (int d = 0; d < ND; ++d)
-                if (g == d % 4) sh.fold[1][j * D + 16 * d + c] = acc[d][j];
-        wave_sync();
-#pragma unroll
-        for (int j = 0; j < NR; ++j)
-            if (j < p.N && 4 * lane < D)
-                put_row<TQ, D>(p, whole, part, b, h, j, 4 * lane, *reinterpret_cast<const f32x4 *>(&sh.fold[1][j * D + 4 * lane]), m[j], l[j]);
-        if (!whole && p.npchunk == 0) {
-            stores_done();
-            if (lane == 0) sh.done = last_part(p, b, h);
-        }
-    }
-    if (whole || p.npchunk > 0) return;
-    __syncthreads();
-    if (sh.done) join_parts<TQ, D, 64 * NW>(p, b, h, sh.join);
-}
-
-// ---------------------------------------------------------------------------
-// wide
-// ---------------------------------------------------------------------------
-template <typename TQ, typename TS, int D, int NC> constexpr int wide_keys() {
-    return D * (int)sizeof(TS) <= 128 && D * (int)sizeof(TQ) <= 256 && NC == 1 ? 64 : D * (int)sizeof(TS) * NC <= 256 ? 32 : 16;
-}
-
-template <typename TQ, typename TS, int D, int NC, bool PRE, typename SH>
-__device__ __forceinline__ void wide_rows(const AttendParams &p, int b0, int h, int tile, int part, SH &sh) {
-    typedef typename Quad<TQ>::t quad_t;
-    constexpr int DG = D / 4, ND = D / 16, ROWS = tile_rows<NC>(), NW = waves(D);
-    // Keys of a step: as many of a page as leave room for the operands of the next step (KT * D * sizeof(TS) / 256 registers
-    // each for K and V), the accumulators and the queries.
-    constexpr int KT = wide_keys<TQ, TS, D, NC>(), KL = KT / 4, A = KT / 16, HT = PG / KT;  // KL of a lane, HT steps a page
-    static_assert(PRE || NC == 1, "a sequence's own rows in tiles of 16");
-    const int tid = thread_x(), lane = tid % 64, wave = uni(tid / 64), c = lane % 16, g = lane / 16;
-    const int H = p.c.H;
-    bool missing = false;                 // a page of the segment that its table does not name: every row's
-    bool bad[NC];                         // of the lane's row
-    bool valid[NC];
-    int sb[NC], si[NC], last[NC];         // sequence, query, last position of the segment that the row sees (-1: none)
-    int npg, pf, lmax, sees_all;          // pages of the segment, pages that every row sees whole, the largest `last`; positions all rows see
-    const int32_t *table;
-    const int64_t rows = PRE ? (int64_t)p.B * p.N : p.N;
-    if constexpr (PRE) {
-        table = p.prefix;
-        npg = (p.PL + PG - 1) / PG;
-        sees_all = p.PL;
-        lmax = p.PL - 1;
-    } else {
-        table = p.table + (int64_t)b0 * p.stable;
-        const int L = uni(seq_len(p, b0, missing)), tmin = L - p.N + tile * ROWS;
-        lmax = min(tmin + ROWS, L) - 1;
-        npg = lmax >= 0 ? lmax / PG + 1 : 0;
-        sees_all = tmin >= 0 ? tmin + 1 : 0;
-    }
-    pf = sees_all / PG;
-    const int chunk = PRE ? p.pchunk : p.chunk;
-    const int ps = part * chunk, pe = min(ps + chunk, npg);
-    const int per = pe > ps ? (pe - ps + NW - 1) / NW : 0;
-    const int ws = ps + wave * per, we = min(ws + per, pe);
-    const int pages = page_numbers(p, table, ws, we, lane, missing);
-    const bool far = pf > ps + PG;
-    const int behind_page = page_numbers(p, table, we, ws < we ? (far ? min(pe, pf) : pf) : 0, lane, missing);
-    const int part_page = page_numbers(p, table, max(we, pf), ws < we ? npg : 0, lane, missing);
-    float mine = we + lane < (far ? min(pe, pf) : pf) && ws < we ? p.c.phi_min[(int64_t)behind_page * H + h] : pinf();
-    auto head_page = [&](int pg) { return (int64_t)__builtin_amdgcn_readlane(pages, pg - ws) * H + h; };
-
-    // step T: keys KT T .. KT T + KT - 1 of the segment
-    Raw<TS, DG> kr[A];
-    Raw<TS, KL> vr[ND];
-    f32x4 phv[A], psv[A];
-    Raw<e4m3, KL> kew, vew;
-    auto place = [&](int T) { return head_page(T / HT) * PG + T % HT * KT; };  // the step's first position in the pool, for this head
-    auto load_k = [&](int64_t at) __attribute__((always_inline)) {
-        const TS *kp = static_cast<const TS *>(p.c.k) + at * D;
-#pragma unroll
-        for (int a = 0; a < A; ++a) kr[a].load(kp + (KL * (c / 4) + 4 * a + c % 4) * D + g * DG);
-    };
-    auto load_s = [&](int64_t at) __attribute__((always_inline)) {
-        if constexpr (sizeof(TS) == 1) {
-            kew.load(reinterpret_cast<const e4m3 *>(p.c.k_exp + at) + KL * g);
-            vew.load(reinterpret_cast<const e4m3 *>(p.c.v_exp + at) + KL * g);
-        }
-#pragma unroll
-        for (int a = 0; a < A; ++a) {
-            phv[a] = *reinterpret_cast<const f32x4 *>(p.c.phi + at + KL * g + 4 * a);
-            psv[a] = *reinterpret_cast<const f32x4 *>(p.c.psi + at + KL * g + 4 * a);
-        }
-    };
-    auto load_v = [&](int64_t at) __attribute__((always_inline)) {
-        const TS *vp = static_cast<const TS *>(p.c.v) + at / PG * (PG * D) + at % PG;
-#pragma unroll
-        for (int d = 0; d < ND; ++d) vr[d].load(vp + (16 * d + c) * PG + KL * g);
-    };
-    const int T0 = ws * HT, T1 = min(we * HT, lmax >= 0 ? lmax / KT + 1 : 0);  // the wave's steps
-    if (T0 < T1) {
-        const int64_t at = place(T1 - 1);
-        load_k(at);
-        load_s(at);
-        load_v(at);
-    }
-
-    quad_t qv[NC][DG / 4];
-    float carry[NC];
-#pragma unroll
-    for (int k = 0; k < NC; ++k) {
-        const int64_t col = (int64_t)tile * ROWS + k * CW + c;
-        valid[k] = col < rows;
-        sb[k] = PRE ? (valid[k] ? (int)(col / p.N) : 0) : b0;
-        si[k] = valid[k] ? (int)(PRE ? col % p.N : col) : 0;
-        bad[k] = false;
-        const int t = seq_len(p, sb[k], bad[k]) - p.N + si[k];
-        last[k] = valid[k] && t >= 0 ? (PRE ? lmax : t) : -1;
-        Raw<TQ, DG> r;
-        r.load(static_cast<const TQ *>(p.q) + (int64_t)sb[k] * p.sq.b + (int64_t)h * p.sq.h + (int64_t)si[k] * p.sq.t + g * DG);
-#pragma unroll
-        for (int i = 0; i < DG / 4; ++i) qv[k][i] = quad<TQ>(r, i);  // columns past the rows repeat one: never written
-        carry[k] = pinf();
-        if constexpr (PRE) {  // min of the sequence's own phi up to t, the lane groups taking the whole pages in turn
-            const int32_t *tb = p.table + (int64_t)sb[k] * p.stable;
-            const int full = t >= 0 ? (t + 1) / PG : 0, rest = t >= 0 ? (t + 1) % PG : 0;
-            carry[k] = lane_min(p, tb, h, g, full, 4, bad[k]);
-            if (rest > 0) {
-                const int page = tb[full];
-                const bool there = (uint32_t)page < (uint64_t)p.c.n;
-                bad[k] |= !there;
-                const float *ph = p.c.phi + ((int64_t)(there ? page : 0) * H + h) * PG + 16 * g;
-#pragma unroll
-                for (int e = 0; e < 16; e += 4) {
-                    const f32x4 f = *reinterpret_cast<const f32x4 *>(ph + e);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        if (16 * g + e + j < rest) carry[k] = fminf(carry[k], f[j]);
-                }
-            }
-        }
-    }
-    const float beta2 = p.beta[h] * LOG2E;
-    {
-        mine = wave_min(mine);
-        if (far) {
-            const float mb = wave_min(lane_min(p, table, h, pe + tid, pf, 64 * NW, missing));
-            if (lane == 0) sh.behind[wave] = mb;
-            __syncthreads();
-#pragma unroll
-            for (int i = 0; i < NW; ++i) mine = fminf(mine, sh.behind[i]);
-        }
-        if (ws < we) {
-            for (int k = max(we, pf); k < npg; ++k) {  // at most two pages that some rows see in part
-                const float *ph = p.c.phi + ((int64_t)__builtin_amdgcn_readlane(part_page, k - max(we, pf)) * H + h) * PG + 16 * g;
-#pragma unroll
-                for (int e = 0; e < 16; e += 4) {
-                    const f32x4 f = *reinterpret_cast<const f32x4 *>(ph + e);
-#pragma unroll
-                    for (int q = 0; q < NC; ++q)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            if (k * PG + 16 * g + e + j <= last[q]) carry[q] = fminf(carry[q], f[j]);
-                }
-            }
-        }
-#pragma unroll
-        for (int k = 0; k < NC; ++k) carry[k] = fminf(min_groups(carry[k]), mine);
-    }
-
-    f32x4 acc[NC][ND];
-    float m[NC], l[NC];
-#pragma unroll
-    for (int k = 0; k < NC; ++k) {
-        m[k] = ninf();
-        l[k] = 0.f;
-#pragma unroll
-        for (int d = 0; d < ND; ++d) acc[k][d] = f32x4{0.f, 0.f, 0.f, 0.f};
-    }
-
-    auto step = [&](auto tail_tag, int T) __attribute__((always_inline)) {
-        constexpr bool TAIL = decltype(tail_tag)::value;
-        const int key0 = T * KT + KL * g;  // the lane's first key
-        const int64_t next = T > T0 ? place(T - 1) : 0;
-        f32x4 s[NC][A];
-#pragma unroll
-        for (int a = 0; a < A; ++a) {
-            quad_t kq[DG / 4];
-#pragma unroll
-            for (int i = 0; i < DG / 4; ++i) kq[i] = quad<TQ>(kr[a], i);
-#pragma unroll
-            for (int k = 0; k < NC; ++k) s[k][a] = mma<DG / 4>(kq, qv[k], f32x4{0.f, 0.f, 0.f, 0.f});
-        }
-        if (T > T0) load_k(next);
-        // range minima of the lane's keys, last to first; what the other groups and steps hold behind them
-        float t[NC][KL];
-        float x[KL], behind = 0.f, all = 0.f;  // outside the tail the same for every row
-#pragma unroll
-        for (int k = 0; k < NC; ++k) {
-            if (TAIL || k == 0) {
-                float r = pinf();
-#pragma unroll
-                for (int e = KL - 1; e >= 0; --e) {
-                    x[e] = fminf(r - psv[e / 4][e % 4], 0.f);
-                    r = fminf(r, (!TAIL || key0 + e <= last[k]) ? phv[e / 4][e % 4] : pinf());
-                }
-                const float r1 = __shfl_down(r, 16, 64), r2 = __shfl_down(r, 32, 64), r3 = __shfl_down(r, 48, 64);
-                behind = pinf();
-                if (g < 3) behind = r1;
-                if (g < 2) behind = fminf(behind, r2);
-                if (g < 1) behind = fminf(behind, r3);
-                all = __shfl(fminf(behind, r), c, 64);
-            }
-            const float low = fminf(behind, carry[k]);
-            carry[k] = fminf(carry[k], all);
-#pragma unroll
-            for (int e = 0; e < KL; ++e) {
-                float sc = p.sc2;
-                if constexpr (sizeof(TS) == 1) sc *= pow2((int)(int8_t)(kew.w[e / 4] >> (8 * (e % 4))));
-                float z = s[k][e / 4][e % 4] * sc;
-                if constexpr (sizeof(TS) == 1) z += (float)(int8_t)(vew.w[e / 4] >> (8 * (e % 4)));
-                t[k][e] = z + beta2 * fminf(x[e], low - psv[e / 4][e % 4]);
-                if (TAIL && key0 + e > last[k]) t[k][e] = ninf();
-            }
-        }
-        float vinv[KL];
-        if constexpr (sizeof(TS) == 1) {
-#pragma unroll
-            for (int e = 0; e < KL; ++e) vinv[e] = pow2(-(int)(int8_t)(vew.w[e / 4] >> (8 * (e % 4))));
-        }
-        if (T > T0) load_s(next);
-        quad_t pq[NC][A];
-#pragma unroll
-        for (int k = 0; k < NC; ++k) {
-            float mt = t[k][0];
-#pragma unroll
-            for (int e = 1; e < KL; ++e) mt = fmaxf(mt, t[k][e]);
-            if (__any(mt > m[k] + SLACK)) {  // rare after the first steps
-                const float mn = fmaxf(m[k], max_groups(mt)), alpha = exp_or_0(m[k], mn);
-                m[k] = mn;
-                l[k] *= alpha;
-#pragma unroll
-                for (int d = 0; d < ND; ++d)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) acc[k][d][j] *= alpha;
-            }
-            const float ref = m[k] == ninf() ? 0.f : m[k];
-#pragma unroll
-            for (int e = 0; e < KL; ++e) {
-                t[k][e] = fexp2(t[k][e] - ref);
-                if constexpr (sizeof(TS) == 1)
-                    l[k] += t[k][e] * vinv[e];
-                else
-                    l[k] += t[k][e];
-                pq[k][e / 4][e % 4] = (TQ)t[k][e];
-            }
-        }
-        bool some = false;
-#pragma unroll
-        for (int d = 0; d < ND; ++d) {
-            if constexpr (TAIL) some |= clean<PRE>(vr[d], lmax + 1 - key0);
-            quad_t vq[A];
-#pragma unroll
-            for (int a = 0; a < A; ++a) vq[a] = quad<TQ>(vr[d], a);
-#pragma unroll
-            for (int k = 0; k < NC; ++k) acc[k][d] = mma<A>(vq, pq[k], acc[k][d]);
-        }
-        if (TAIL && !PRE && __any(some)) {  // infinities and NaN, for the rows that see them
-            const int64_t at = place(T);
-            const TS *vp = static_cast<const TS *>(p.c.v) + at / PG * (PG * D) + at % PG;
-            for (int e = 0; e < KT; ++e) {
-                float w = t[0][0];
-#pragma unroll
-                for (int k = 1; k < KL; ++k) w = e % KL == k ? t[0][k] : w;
-                w = __shfl(w, e / KL * 16 + c, 64);
-#pragma unroll
-                for (int d = 0; d < ND; ++d)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const float y = not_finite(vp + (16 * d + 4 * g + j) * PG + e);
-                        if (T * KT + e <= last[0] && __float_as_uint(y) != 0) acc[0][d][j] += w * y;
-                    }
-            }
-        }
-        if (T > T0) load_v(next);
-    };
-    int T = T1 - 1;
-    for (; T >= T0 && (T + 1) * KT > sees_all; --T) step(std::true_type{}, T);
-    for (; T >= T0; --T) step(std::false_type{}, T);
-
-    const bool lost = __any(missing);
-#pragma unroll
-    for (int k = 0; k < NC; ++k) {
-        l[k] = sum_groups(l[k]);
-        if (last[k] < 0) {  // a row that sees nothing: whole pages are not masked for it
-            m[k] = ninf();
-            l[k] = 0.f;
-#pragma unroll
-            for (int d = 0; d < ND; ++d) acc[k][d] = f32x4{0.f, 0.f, 0.f, 0.f};
-        }
-        if (lost || max_groups(bad[k] ? 1.f : 0.f) > 0.f) l[k] = __uint_as_float(BAD);
-    }
-    // The waves' results together, the upper half into the lower, down to wave 0 (lane by lane: every wave has the same rows).
-#pragma unroll
-    for (int from = NW / 2; from >= 1; from /= 2) {
-        __syncthreads();
-        if (wave >= from && wave < 2 * from) {
-#pragma unroll
-            for (int k = 0; k < NC; ++k) {
-                if (g == 0) {
-                    sh.stat[wave - from][2 * (k * CW + c)] = m[k];
-                    sh.stat[wave - from][2 * (k * CW + c) + 1] = l[k];
-                }
-#pragma unroll
-                for (int d = 0; d < ND; ++d) *reinterpret_cast<f32x4 *>(&sh.fold[wave - from][((k * ND + d) * 64 + lane) * 4]) = acc[k][d];
-            }
-        }
-        __syncthreads();
-        if (wave < from) {
-#pragma unroll
-            for (int k = 0; k < NC; ++k) {
-                const float m2 = sh.stat[wave][2 * (k * CW + c)], l2 = sh.stat[wave][2 * (k * CW + c) + 1], mn = fmaxf(m[k], m2);
-                const float a = exp_or_0(m[k], mn), w = exp_or_0(m2, mn);
-                const bool b2 = __float_as_uint(l[k]) == BAD || __float_as_uint(l2) == BAD;
-                m[k] = mn;
-                l[k] = b2 ? __uint_as_float(BAD) : l[k] * a + l2 * w;
-#pragma unroll
-                for (int d = 0; d < ND; ++d) {
-                    const f32x4 o = *reinterpret_cast<const f32x4 *>(&sh.fold[wave][((k * ND + d) * 64 + lane) * 4]);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) acc[k][d][j] = acc[k][d][j] * a + o[j] * w;
-                }
-            }
-        }
-    }
-    bool over = false;
-    const bool whole = !PRE && p.npchunk == 0 && own_parts(p, uni(seq_len(p, b0, over))) == 1;
-    if (wave == 0) {
-#pragma unroll
-        for (int k = 0; k < NC; ++k)
-            if (valid[k]) {
-#pragma unroll
-                for (int d = 0; d < ND; ++d)
-                    put_row<TQ, D>(p, whole, PRE ? p.nchunk + part : part, sb[k], h, si[k], 16 * d + 4 * g, acc[k][d], m[k], l[k]);
-            }
-        if (!whole && p.npchunk == 0) {
-            stores_done();
-            if (lane == 0) sh.done = last_part(p, b0, h);
-        }
-    }
-    if (whole || p.npchunk > 0) return;
-    __syncthreads();
-    if (sh.done) join_parts<TQ, D, 64 * NW>(p, b0, h, sh.join);
-}
-
-// With a prefix: its parts belong to the rows of many sequences, which one last workgroup would join one after the other.
-template <typename TQ, int D> __global__ __launch_bounds__(256) void fpa_attend_join_kernel(AttendParams p) {
-    __shared__ float join[256][6];
-    join_parts<TQ, D, 256>(p, group_x() / p.c.H, group_x() % p.c.H, join);
-}
-// KIND 1, 4: own rows by the few form with that many; 0: by the wide form.  NC: 16-row sets of the prefix's tiles (0: no prefix).
-template <typename TQ, typename TS, int D, int KIND, int NC> __global__ __launch_bounds__(64 * waves(D)) void fpa_attend_kernel(AttendParams p) {
-    __shared__ __align__(16) Shared<D, (NC ? NC : 1)> sh;
-    __shared__ __align__(16) TQ weights[KIND ? waves(D) : 1][KIND ? KIND * PG : 1];
-    int64_t id = group_x();
-    const int H = p.c.H;
-    if constexpr (NC > 0) {
-        constexpr int ROWS = tile_rows<NC>();
-        const int tiles = (int)(((int64_t)p.B * p.N + ROWS - 1) / ROWS);
-        // Tiles of the same pages run on one XCD (workgroups go to the eight in turn), one after the other, so that its L2 has
-        // what the first of them read.
-        const int64_t units = (int64_t)p.npchunk * H, npre = (units + 7) / 8 * 8 * tiles;
-        if (id < npre) {
-            const int64_t unit = id / (8 * tiles) * 8 + id % 8;
-            if (unit < units)
-                wide_rows<TQ, TS, D, NC, true>(p, 0, (int)(unit / p.npchunk), (int)(id / 8 % tiles), (int)(unit % p.npchunk), sh);
-            return;
-        }
-        id -= npre;
-    }
-    const int nrt = (p.N + CW - 1) / CW;  // tiles of a sequence's rows
-    const int tile = (int)(id % nrt);
-    id /= nrt;
-    const int bh = (int)(id % ((int64_t)p.B * H)), part = (int)(id / ((int64_t)p.B * H));
-    const int b = bh / H, h = bh % H;
-    bool lost = false;
-    if (part >= own_parts(p, seq_len(p, b, lost))) return;
-    if constexpr (KIND > 0)
-        few_rows<TQ, TS, D, KIND>(p, b, h, part, sh, weights);
-    else
-        wide_rows<TQ, TS, D, 1, false>(p, b, h, tile, part, sh);
-}
-
-// Row tiles of the prefix: 32 rows where there are more than 16 and their accumulators fit (fp16 to D = 128, fp32 to 64).
-constexpr bool two_sets(int D, bool f32) { return D <= (f32 ? 64 : 128); }
-int prefix_sets(int D, int64_t rows, bool f32) { return rows > CW && two_sets(D, f32) ? 2 : 1; }
-
-template <typename TQ, typename TS, int D> hipError_t launch_attend_d(const AttendParams &p, hipStream_t s) {
-    const int64_t rows = (int64_t)p.B * p.N, H = p.c.H;
-    const int sets = prefix_sets(D, rows, sizeof(TQ) == 4), trows = CW * sets;
-    const int64_t pre = (p.npchunk * H + 7) / 8 * 8 * ((rows + trows - 1) / trows);
-    const int64_t own = (int64_t)p.nchunk * p.B * H * ((p.N + CW - 1) / CW);
-    const dim3 grid((uint32_t)(pre + own)), block(64 * waves(D));
-    if (p.npchunk == 0) {
-        if (p.N == 1)
-            hipLaunchKernelGGL((fpa_attend_kernel<TQ, TS, D, 1, 0>), grid, block, 0, s, p);
-        else if (p.N <= 4)
-            hipLaunchKernelGGL((fpa_attend_kernel<TQ, TS, D, 4, 0>), grid, block, 0, s, p);
-        else
-            hipLaunchKernelGGL((fpa_attend_kernel<TQ, TS, D, 0, 0>), grid, block, 0, s, p);
-    } else if (sets == 1) {
-        if (p.N <= 4)
-            hipLaunchKernelGGL((fpa_attend_kernel<TQ, TS, D, 4, 1>), grid, block, 0, s, p);
-        else
-            hipLaunchKernelGGL((fpa_attend_kernel<TQ, TS, D, 0, 1>), grid, block, 0, s, p);
-    } else if constexpr (two_sets(D, sizeof(TQ) == 4)) {
-        if (p.N <= 4)
-            hipLaunchKernelGGL((fpa_attend_kernel<TQ, TS, D, 4, 2>), grid, block, 0, s, p);
-        else
-            hipLaunchKernelGGL((fpa_attend_kernel<TQ, TS, D, 0, 2>), grid, block, 0, s, p);
-    }
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess || p.npchunk == 0) return e;
-    hipLaunchKernelGGL((fpa_attend_join_kernel<TQ, D>), dim3((uint32_t)(p.B * H)), dim3(256), 0, s, p);
-    return hipGetLastError();
-}
-
-template <typename TQ, typename TS> hipError_t launch_attend_t(const AttendParams &p, int D, hipStream_t s) {
-    switch (D) {
-        case 16: return launch_attend_d<TQ, TS, 16>(p, s);
-        case 32: return launch_attend_d<TQ, TS, 32>(p, s);
-        case 64: return launch_attend_d<TQ, TS, 64>(p, s);
-        case 128: return launch_attend_d<TQ, TS, 128>(p, s);
-        case 256: return launch_attend_d<TQ, TS, 256>(p, s);
-    }
-    return hipErrorInvalidValue;
-}
-
-}  // namespace
+extern template hipError_t launch_attend_small<f16, f16>(const AttendParams &, int, hipStream_t);
+extern template hipError_t launch_attend_large<f16, f16>(const AttendParams &, int, hipStream_t);
+extern template hipError_t launch_attend_small<float, float>(const AttendParams &, int, hipStream_t);
+extern template hipError_t launch_attend_large<float, float>(const AttendParams &, int, hipStream_t);
+extern template hipError_t launch_attend_small<f16, e4m3>(const AttendParams &, int, hipStream_t);
+extern template hipError_t launch_attend_large<f16, e4m3>(const AttendParams &, int, hipStream_t);
+extern template hipError_t launch_attend_small<float, e4m3>(const AttendParams &, int, hipStream_t);
+extern template hipError_t launch_attend_large<float, e4m3>(const AttendParams &, int, hipStream_t);
 
 hipError_t launch_attend(const AttendParams &p, int dtype, int store, int D, hipStream_t s) {
-    if (dtype == ST_F16 && store == ST_F16) return launch_attend_t<f16, f16>(p, D, s);
-    if (dtype == ST_F32 && store == ST_F32) return launch_attend_t<float, float>(p, D, s);
-    if (dtype == ST_F16 && store == ST_E4M3) return launch_attend_t<f16, e4m3>(p, D, s);
-    if (dtype == ST_F32 && store == ST_E4M3) return launch_attend_t<float, e4m3>(p, D, s);
+    if (dtype == ST_F16 && store == ST_F16) return D <= 64 ? launch_attend_small<f16, f16>(p, D, s) : launch_attend_large<f16, f16>(p, D, s);
+    if (dtype == ST_F32 && store == ST_F32) return D <= 64 ? launch_attend_small<float, float>(p, D, s) : launch_attend_large<float, float>(p, D, s);
+    if (dtype == ST_F16 && store == ST_E4M3) return D <= 64 ? launch_attend_small<f16, e4m3>(p, D, s) : launch_attend_large<f16, e4m3>(p, D, s);
+    if (dtype == ST_F32 && store == ST_E4M3) return D <= 64 ? launch_attend_small<float, e4m3>(p, D, s) : launch_attend_large<float, e4m3>(p, D, s);
     return hipErrorInvalidValue;
 }
+
+int attend_waves(int D) { return waves(D); }
 
 int attend_rows(int64_t rows, int D, int dtype) { return CW * prefix_sets(D, rows, dtype == ST_F32); }
 
-void attend_parts(int64_t items, int64_t pages, int D, int &chunk, int &nchunk) {
 #ifndef PARTS_WG
-#define PARTS_WG 1024
+#define PARTS_WG 256
 #endif
-    const int nw = waves(D);
-    const int64_t want = items >= PARTS_WG ? 1 : (PARTS_WG + items - 1) / items;
-    int64_t c = ((pages + want - 1) / want + nw - 1) / nw * nw;  // the same for every wave, one page at least
-    c = c > 64 ? 64 : c;  // long sequences among short ones are spread in any case
+#ifndef ALONE_PAGES
+#define ALONE_PAGES 16
+#define ALONE_ITEMS 256
+#endif
+
+int attend_steps(int D, int dtype, int store, int64_t N, bool prefix, int sets) {
+    const int kind = N > 4 ? 0 : N > 1 || prefix ? 4 : 1;
+    if (store == ST_F16) return steps_of<f16, f16>(D, kind, sets);
+    if (store == ST_F32) return steps_of<float, float>(D, kind, sets);
+    return dtype == ST_F16 ? steps_of<f16, e4m3>(D, kind, sets) : steps_of<float, e4m3>(D, kind, sets);
+}
+
+void attend_parts(int64_t items, int64_t pages, int D, int steps, int64_t taken, int &chunk, int &nchunk) {
+    // As many parts as fill the CUs once, beside the `taken` workgroups that run with them: a workgroup's start and end cost as
+    // much as several pages.  At most 64 pages, so that long sequences among short ones are spread in any case.
+    const int least = waves(D) / steps > 1 ? waves(D) / steps : 1;  // one step a wave
+    const int64_t room = PARTS_WG - taken > PARTS_WG / 2 ? PARTS_WG - taken : PARTS_WG / 2;
+    const int64_t want = items >= room ? 1 : room / items;
+    int64_t c = ((pages + want - 1) / want + least - 1) / least * least;  // the same for every wave
+    c = c > 64 ? 64 : c;
     chunk = (int)c;
     nchunk = (int)((pages + c - 1) / c);
+}
+
+bool attend_alone(int64_t B, int64_t H, int64_t N, int64_t pages, int D, int dtype, bool prefix) {
+    return pages <= ALONE_PAGES && B * H >= ALONE_ITEMS && alone_built(N <= 4 ? 4 : 0, prefix ? prefix_sets(D, B * N, dtype == ST_F32) : 0);
 }
 
 }  // namespace fpa

@@ -157,7 +157,9 @@ def lib():
         getattr(L, name).restype = ctypes.c_int
         getattr(L, name).argtypes = [ctypes.POINTER(args), _vp]
     L.fpa_attend_workspace_bytes.restype = _i64
-    L.fpa_attend_workspace_bytes.argtypes = [_i64] * 6 + [ctypes.c_int32]
+    L.fpa_attend_workspace_bytes.argtypes = [_i64] * 6 + [ctypes.c_int32] * 2
+    L.fpa_attend_counts.restype = _i64
+    L.fpa_attend_counts.argtypes = [_i64] * 3
     L.fpa_verify_workspace_bytes.restype = _i64
     L.fpa_verify_workspace_bytes.argtypes = [_i64] * 2
     if L.fpa_abi_version() != ABI_VERSION:

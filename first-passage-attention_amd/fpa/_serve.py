@@ -58,8 +58,10 @@ def read(c, table, start, n, counts, dtype):
 
 
 @functools.lru_cache(maxsize=256)
-def _attend_ws_bytes(B, H, N, D, P, prefix_length, dtype):
-    return _lib.lib().fpa_attend_workspace_bytes(B, H, N, D, P, prefix_length, dtype)
+def _attend_scratch(B, H, N, D, P, prefix_length, dtype, store):
+    """(workspace bytes, counters) of a call of this shape."""
+    L = _lib.lib()
+    return L.fpa_attend_workspace_bytes(B, H, N, D, P, prefix_length, dtype, store), L.fpa_attend_counts(B, H, N)
 
 
 def attend(q, c, beta, table, lengths, prefix, prefix_length):
@@ -70,12 +72,12 @@ def attend(q, c, beta, table, lengths, prefix, prefix_length):
     P = table.shape[1]
     with device_guard(dev):
         o = torch.empty((B, N, H, D), dtype=q.dtype, device=dev).transpose(1, 2)
-        nws = _attend_ws_bytes(B, H, N, D, P, prefix_length, _CODES[q.dtype])
+        nws, ncounts = _attend_scratch(B, H, N, D, P, prefix_length, _CODES[q.dtype], _CODES[c.dtype])
         ws = workspace(dev, nws) if nws else None
         a = _lib.FpaAttendArgs.from_buffer_copy(_lib.ATTEND_PACK.pack(
             _pages(c), B, N, P, _CODES[q.dtype], q.data_ptr(), *q.stride(), o.data_ptr(), *o.stride(), beta.data_ptr(),
             table.data_ptr(), table.stride(0), lengths.data_ptr(), _ptr(prefix), prefix_length, _ptr(ws),
-            counters(dev, B * H).data_ptr()))
+            counters(dev, ncounts).data_ptr()))
         _lib.check(_lib.lib().fpa_attend(a, _lib.stream_of(dev)))
     return o
 

@@ -264,11 +264,13 @@ typedef struct {
     const int32_t *prefix;                 /* or NULL */
     int64_t prefix_length;
     void *workspace;                       /* fpa_attend_workspace_bytes(), 256-byte aligned */
-    int32_t *counts;                       /* B * H ints of device memory, zero before the first call; every call
+    int32_t *counts;                       /* fpa_attend_counts() ints of device memory, zero before the first call; every call
                                               leaves them zero.  Calls that may overlap need counts of their own,
                                               as they need workspaces of their own. */
 } FpaAttendArgs;
-int64_t fpa_attend_workspace_bytes(int64_t B, int64_t H, int64_t N, int64_t D, int64_t P, int64_t prefix_length, int32_t dtype);
+int64_t fpa_attend_workspace_bytes(int64_t B, int64_t H, int64_t N, int64_t D, int64_t P, int64_t prefix_length, int32_t dtype,
+                                   int32_t store);
+int64_t fpa_attend_counts(int64_t B, int64_t H, int64_t N);
 int fpa_attend(const FpaAttendArgs *args, void *stream);
 
 /* Verifies N drafted tokens of B sequences.  target: probabilities (B, N + 1, V), draft: (B, N, V) or NULL for

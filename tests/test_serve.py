@@ -291,7 +291,7 @@ def test_serving_c_abi_null_and_sizes():
     assert L.fpa_verify(a, None) == _lib.FPA_ERR_INVALID and "non-NULL" in L.fpa_last_error().decode()
     a.V = 2 ** 31
     assert L.fpa_verify(a, None) == _lib.FPA_ERR_UNSUPPORTED
-    assert L.fpa_attend_workspace_bytes(1, 2, 1, 64, 1, 0, 0) == 0
-    n = L.fpa_attend_workspace_bytes(1, 2, 1, 64, 100, 0, 0)
+    assert L.fpa_attend_workspace_bytes(1, 2, 1, 64, 1, 0, 0, 0) == 0
+    n = L.fpa_attend_workspace_bytes(1, 2, 1, 64, 100, 0, 0, 0)
     assert n > 0 and n % 256 == 0
     assert tables([1], 1, 1, torch.Generator().manual_seed(0)).tolist() == [[0]]
