@@ -443,26 +443,28 @@ Pages pages_of(const FpaPages &c) {
 
 // Parts of the sequences' own pages and of the prefix, and their scratch.
 struct AttendPlan {
-    int chunk, nchunk, pchunk = 1, npchunk = 0;
+    int nchunk, pchunk = 1, npchunk = 0, least = 1, slots = 1;
     bool alone;
+    int64_t groups;  // workgroups for the sequences' own pages
     int64_t ml, total;  // float offset of the statistics, bytes
 };
 AttendPlan attend_plan(int64_t B, int64_t H, int64_t N, int64_t D, int64_t P, int64_t PL, int32_t dtype, int32_t store) {
     AttendPlan a;
     const int64_t rows = attend_rows(B * N, (int)D, dtype);
-    const int64_t items = B * H * ((N + 15) / 16);
+    const int64_t units = H * ((N + 15) / 16), nw = attend_waves((int)D);
     a.alone = attend_alone(B, H, N, P, (int)D, dtype, PL > 0);
     if (a.alone) {
-        a.chunk = (int)P;
         a.nchunk = 1;
+        a.groups = (B * units + nw - 1) / nw;
     } else {
-        attend_parts(items, P, (int)D, attend_steps((int)D, dtype, store, N, PL > 0, 0), 0, a.chunk, a.nchunk);
+        attend_own(B, units, P, (int)D, attend_steps((int)D, dtype, store, N, PL > 0, 0),
+                   (int)(2 * PG * D * (store == FPA_F32 ? 4 : store == FPA_F16 ? 2 : 1)), PL > 0, a.least, a.slots, a.nchunk, a.groups);
     }
     if (PL > 0) attend_parts(H * ((B * N + rows - 1) / rows), (PL + PG - 1) / PG, (int)D, attend_steps((int)D, dtype, store, N, true, (int)rows / 16),
-                             a.alone ? (B * H + attend_waves((int)D) - 1) / attend_waves((int)D) : items * a.nchunk, a.pchunk, a.npchunk);
-    const int64_t slots = (a.nchunk <= 1 && a.npchunk == 0) ? 0 : (int64_t)(a.nchunk + a.npchunk) * B * H * N;
-    a.ml = align64(slots * D);
-    a.total = (a.ml + align64(slots * 2)) * (int64_t)sizeof(float);
+                             a.groups, a.pchunk, a.npchunk);
+    const int64_t parts = (a.nchunk <= 1 && a.npchunk == 0) ? 0 : (int64_t)(a.nchunk + a.npchunk) * B * H * N;
+    a.ml = align64(parts * D);
+    a.total = (a.ml + align64(parts * 2)) * (int64_t)sizeof(float);
     return a;
 }
 
@@ -547,7 +549,9 @@ int fpa_attend(const FpaAttendArgs *a, void *stream) {
     p.ml = p.part + pl.ml;
     p.counts = a->counts;
     p.B = (int)a->B; p.N = (int)a->N; p.P = (int)a->P; p.PL = (int)a->prefix_length;
-    p.chunk = pl.chunk; p.nchunk = pl.nchunk; p.pchunk = pl.pchunk; p.npchunk = pl.npchunk; p.alone = pl.alone;
+    p.chunk = (int)a->P;  // of a wave that takes a sequence alone
+    p.nchunk = pl.nchunk; p.pchunk = pl.pchunk; p.npchunk = pl.npchunk; p.alone = pl.alone;
+    p.least = pl.least; p.slots = pl.slots; p.own_groups = pl.groups;
     p.sc2 = LOG2E / sqrtf((float)D);
     const hipError_t e = launch_attend(p, a->dtype, a->cache.store, (int)D, reinterpret_cast<hipStream_t>(stream));
     return e != hipSuccess ? hip_fail(e, "fpa_attend launch") : FPA_OK;

@@ -58,12 +58,13 @@ template <typename TS, int N> struct Raw {
     static constexpr int BYTES = N * (int)sizeof(TS);
     static_assert(BYTES % 4 == 0, "whole words");
     uint32_t w[BYTES / 4];
-    __device__ __forceinline__ void load(const TS *p) {
+    // In pieces of 16 bytes (or all of fewer) that lie STRIDE pieces apart.
+    template <int STRIDE> __device__ __forceinline__ void load(const TS *p) {
         const char *b = reinterpret_cast<const char *>(p);
         if constexpr (BYTES % 16 == 0) {
 #pragma unroll
             for (int i = 0; i < BYTES / 16; ++i) {
-                const u32x4 x = *reinterpret_cast<const u32x4 *>(b + 16 * i);
+                const u32x4 x = *reinterpret_cast<const u32x4 *>(b + 16 * STRIDE * i);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) w[4 * i + j] = x[j];
             }
@@ -121,22 +122,22 @@ template <typename TS> __device__ __forceinline__ bool beyond_bits(uint32_t bits
     if constexpr (sizeof(TS) == 2) return (bits & 0x7c00u) == 0x7c00u;
     return (bits & 0x7f800000u) == 0x7f800000u;
 }
-// Word masks that keep the first n of N values.
-template <typename TS, int N> struct Kept {
+// Word masks that keep, of N values in pieces of VL whose positions lie 4 VL apart, those at positions below n (from the first's).
+template <typename TS, int N, int VL> struct Kept {
     static constexpr int PW = 4 / sizeof(TS), BITS = 8 * sizeof(TS);  // values of a word
     uint32_t w[N / PW];
     __device__ __forceinline__ explicit Kept(int n) {
 #pragma unroll
         for (int i = 0; i < N / PW; ++i) {
-            const int k = max(n - i * PW, 0);
+            const int k = max(n - (i * PW / VL * 4 * VL + i * PW % VL), 0);
             w[i] = k >= PW ? 0xffffffffu : (1u << (k * BITS)) - 1u;
         }
     }
 };
 // Clears the values that `kept` leaves out and (unless WHOLE) those that are not finite; `some` gets bits where there were
 // such among the kept.  An exponent of ones carries into the sign's place when one is added to it.
-template <bool WHOLE, typename TS, int N> __device__ __forceinline__ void clean(Raw<TS, N> &r, const Kept<TS, N> &kept, uint32_t &some) {
-    constexpr int PW = Kept<TS, N>::PW;
+template <bool WHOLE, typename TS, int N, int VL> __device__ __forceinline__ void clean(Raw<TS, N> &r, const Kept<TS, N, VL> &kept, uint32_t &some) {
+    constexpr int PW = Kept<TS, N, VL>::PW;
 #pragma unroll
     for (int i = 0; i < N / PW; ++i) {
         r.w[i] &= kept.w[i];
@@ -173,6 +174,21 @@ template <typename TS> __device__ __forceinline__ float not_finite(const TS *vx)
         return beyond_bits<TS>(*reinterpret_cast<const uint16_t *>(vx)) ? (float)*vx : 0.f;
     else
         return beyond_bits<TS>(*reinterpret_cast<const uint32_t *>(vx)) ? *vx : 0.f;
+}
+
+// Features of a lane in the score product: pieces of CH neighbouring ones, 16 bytes of a K row, which the four lane groups take
+// in turn, so that one load of the wave reads 64 bytes of a row in a piece (40% fewer L1 accesses at D = 128 in e4m3 than with a
+// lane's bytes side by side; the same time, which other things bound).
+template <typename TS, int D> constexpr int chunk_of() { return D / 4 < 16 / (int)sizeof(TS) ? D / 4 : 16 / (int)sizeof(TS); }
+template <typename TQ, typename TS, int D> __device__ __forceinline__ void load_query(typename Quad<TQ>::t (&q)[D / 16], const TQ *row, int g) {
+    constexpr int CH = chunk_of<TS, D>();
+#pragma unroll
+    for (int i = 0; i < D / 4 / CH; ++i) {
+        Raw<TQ, CH> r;
+        r.template load<1>(row + CH * (4 * i + g));
+#pragma unroll
+        for (int k = 0; k < CH / 4; ++k) q[i * (CH / 4) + k] = quad<TQ>(r, k);
+    }
 }
 
 // acc += A B^T over NQ quads of the contraction (A: row lane % 16, B: column lane % 16, both of the lane
@@ -302,6 +318,8 @@ template <int NC> constexpr int tile_rows() { return CW * NC; }
 
 // Waves of a workgroup: as many as two a SIMD (their registers end at 256), so that most sequences need no second part.
 constexpr int waves(int D) { return D <= 128 ? 8 : 4; }
+// Pages of a part at most: a wave holds the numbers of its own in one register.
+constexpr int most_pages(int D) { return 48 * waves(D); }
 
 // Parts of a sequence's own pages: one at least, which may be empty.
 __device__ __forceinline__ int own_parts(const AttendParams &p, int L) {
@@ -445,6 +463,7 @@ template <int N, typename F> __device__ __forceinline__ void unrolled(F &&f) {
 template <int NW, int HT, bool ALONE> __device__ __forceinline__ void wave_steps(int ps, int pe, int wave, int &T0, int &T1) {
     const int n = pe > ps ? (pe - ps) * HT : 0, per = ALONE ? n : (n + NW - 1) / NW;
     T0 = ps * HT + (ALONE ? 0 : min(wave * per, n));
+    if constexpr (ALONE) asm("" : "+s"(T0));  // a constant 0 here makes the compiler rearrange the step loops, with hundreds of spills
     T1 = min(T0 + per, ps * HT + n);
 }
 
@@ -525,6 +544,8 @@ __device__ __forceinline__ void few_rows(const AttendParams &p, int b, int h, in
     typedef typename Quad<TQ>::t quad_t;
     constexpr int DG = D / 4, ND = D / 16, NW = waves(D);
     constexpr int KT = few_keys<TQ, TS, D, NR>(), KL = KT / 4, A = KT / 16, HT = PG / KT;
+    constexpr int CH = chunk_of<TS, D>(), VL = KL < 16 / (int)sizeof(TS) ? KL : 16 / (int)sizeof(TS);  // values of a piece of K and V
+    // Value e of a V run is key 4 VL (e / VL) + VL g + e % VL of the step.
     // One fp32 row: the fp32 MFMA would take 15 idle rows along, 8 times the cycles that the same operands take on the vector
     // unit, each lane summing over its own features or keys.
     constexpr bool ONE = sizeof(TQ) == 4 && NR == 1;
@@ -560,7 +581,7 @@ __device__ __forceinline__ void few_rows(const AttendParams &p, int b, int h, in
     auto load_k = [&](int64_t at) __attribute__((always_inline)) {
         const TS *kp = static_cast<const TS *>(p.c.k) + at * D;
 #pragma unroll
-        for (int a = 0; a < A; ++a) kr[a].load(kp + (KT - 1 - 16 * a - c) * D + g * DG);
+        for (int a = 0; a < A; ++a) kr[a].template load<4>(kp + (KT - 1 - 16 * a - c) * D + g * CH);
         phv = p.c.phi[at + key];
         psv = p.c.psi[at + key];
         if constexpr (sizeof(TS) == 1) ke = p.c.k_exp[at + key];
@@ -569,7 +590,7 @@ __device__ __forceinline__ void few_rows(const AttendParams &p, int b, int h, in
         const TS *vp = static_cast<const TS *>(p.c.v) + at / PG * (PG * D) + at % PG;
         if constexpr (sizeof(TS) == 1) ve = p.c.v_exp[at + key];
 #pragma unroll
-        for (int d = 0; d < ND; ++d) vr[d].load(vp + (16 * d + c) * PG + KL * g);
+        for (int d = 0; d < ND; ++d) vr[d].template load<4>(vp + (16 * d + c) * PG + VL * g);
     };
     const int first = min(T1, (L + KT - 1) / KT) - 1;  // steps behind the last position hold nothing
     if (T0 <= first) {
@@ -581,11 +602,8 @@ __device__ __forceinline__ void few_rows(const AttendParams &p, int b, int h, in
     quad_t qv[DG / 4];
     {
         const int i = NR == 1 ? 0 : c % NR;
-        Raw<TQ, DG> r;
-        r.load(static_cast<const TQ *>(p.q) + (int64_t)b * p.sq.b + (int64_t)h * p.sq.h + (int64_t)min(i, p.N - 1) * p.sq.t + g * DG);
-#pragma unroll
-        for (int k = 0; k < DG / 4; ++k) qv[k] = quad<TQ>(r, k);  // rows past N repeat the last: never written
-    }
+        load_query<TQ, TS, D>(qv, static_cast<const TQ *>(p.q) + (int64_t)b * p.sq.b + (int64_t)h * p.sq.h + (int64_t)min(i, p.N - 1) * p.sq.t, g);
+    }  // rows past N repeat the last: never written
     const float beta2 = p.beta[h] * LOG2E;
 
     // min of phi from the wave's pages on: whole pages, those beyond the next 64 by all waves together, then the at most
@@ -713,10 +731,10 @@ __device__ __forceinline__ void few_rows(const AttendParams &p, int b, int h, in
         wave_sync();
         quad_t pq[A];
 #pragma unroll
-        for (int a = 0; a < A; ++a) pq[a] = *reinterpret_cast<const quad_t *>(wl + (NR == 1 ? 0 : c % NR) * PG + KL * g + 4 * a);
+        for (int a = 0; a < A; ++a) pq[a] = *reinterpret_cast<const quad_t *>(wl + (NR == 1 ? 0 : c % NR) * PG + 4 * VL * (4 * a / VL) + VL * g + 4 * a % VL);
         wave_sync();
         uint32_t some = 0;
-        const Kept<TS, KL> kept(TAIL ? L - T * KT - KL * g : KL);
+        const Kept<TS, KL, VL> kept(TAIL ? L - T * KT - VL * g : KT);
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
             if constexpr (TAIL) clean<NR == 1>(vr[d], kept, some);
@@ -834,6 +852,7 @@ __device__ __forceinline__ void wide_rows(const AttendParams &p, int b0, int h, 
     // Keys of a step: as many of a page as leave room for the operands of the next step (KT * D * sizeof(TS) / 256 registers
     // each for K and V), the accumulators and the queries.
     constexpr int KT = wide_keys<TQ, TS, D, NC>(), KL = KT / 4, A = KT / 16, HT = PG / KT;  // KL of a lane, HT steps a page
+    constexpr int CH = chunk_of<TS, D>();
     static_assert(PRE || NC == 1, "a sequence's own rows in tiles of 16");
     const int tid = thread_x(), lane = tid % 64, wave = uni(tid / 64), c = lane % 16, g = lane / 16;
     const int H = p.c.H;
@@ -881,7 +900,7 @@ __device__ __forceinline__ void wide_rows(const AttendParams &p, int b0, int h, 
     auto load_k = [&](int64_t at) __attribute__((always_inline)) {
         const TS *kp = static_cast<const TS *>(p.c.k) + at * D;
 #pragma unroll
-        for (int a = 0; a < A; ++a) kr[a].load(kp + (KL * (c / 4) + 4 * a + c % 4) * D + g * DG);
+        for (int a = 0; a < A; ++a) kr[a].template load<4>(kp + (KL * (c / 4) + 4 * a + c % 4) * D + g * CH);
     };
     auto load_s = [&](int64_t at) __attribute__((always_inline)) {
         const int64_t i = at + KL * g + c % KL;
@@ -895,7 +914,7 @@ __device__ __forceinline__ void wide_rows(const AttendParams &p, int b0, int h, 
     auto load_v = [&](int64_t at) __attribute__((always_inline)) {
         const TS *vp = static_cast<const TS *>(p.c.v) + at / PG * (PG * D) + at % PG;
 #pragma unroll
-        for (int d = 0; d < ND; ++d) vr[d].load(vp + (16 * d + c) * PG + KL * g);
+        for (int d = 0; d < ND; ++d) vr[d].template load<1>(vp + (16 * d + c) * PG + KL * g);
     };
     const int first = min(T1, lmax >= 0 ? lmax / KT + 1 : 0) - 1;  // steps behind the last position hold nothing
     if (T0 <= first) {
@@ -916,10 +935,8 @@ __device__ __forceinline__ void wide_rows(const AttendParams &p, int b0, int h, 
         bad[k] = false;
         const int t = seq_len(p, sb[k], bad[k]) - p.N + si[k];
         last[k] = valid[k] && t >= 0 ? (PRE ? lmax : t) : -1;
-        Raw<TQ, DG> r;
-        r.load(static_cast<const TQ *>(p.q) + (int64_t)sb[k] * p.sq.b + (int64_t)h * p.sq.h + (int64_t)si[k] * p.sq.t + g * DG);
-#pragma unroll
-        for (int i = 0; i < DG / 4; ++i) qv[k][i] = quad<TQ>(r, i);  // columns past the rows repeat one: never written
+        // columns past the rows repeat one: never written
+        load_query<TQ, TS, D>(qv[k], static_cast<const TQ *>(p.q) + (int64_t)sb[k] * p.sq.b + (int64_t)h * p.sq.h + (int64_t)si[k] * p.sq.t, g);
         carry[k] = pinf();
         if constexpr (PRE) {  // min of the sequence's own phi up to t, the lane groups taking the whole pages in turn
             const int32_t *tb = p.table + (int64_t)sb[k] * p.stable;
@@ -1065,7 +1082,7 @@ __device__ __forceinline__ void wide_rows(const AttendParams &p, int b0, int h, 
             });
         }
         uint32_t some = 0;
-        const Kept<TS, KL> kept(TAIL ? lmax + 1 - key0 : KL);
+        const Kept<TS, KL, KL> kept(TAIL ? lmax + 1 - key0 : KT);
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
             if constexpr (TAIL) clean<PRE>(vr[d], kept, some);
@@ -1175,14 +1192,65 @@ __device__ __forceinline__ void wide_rows(const AttendParams &p, int b0, int h, 
     }
 }
 
+__device__ __forceinline__ int wave_sum_i(int x) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) x += __shfl_xor(x, o, 64);
+    return x;
+}
+__device__ __forceinline__ int pages_at(const AttendParams &p, int b) {
+    bool over = false;
+    return b < p.B ? (seq_len(p, b, over) + PG - 1) / PG : 0;
+}
+// Parts of all sequences (`units` workgroups take each: heads and row tiles) for parts of c pages.
+__device__ __forceinline__ int parts_in_all(const AttendParams &p, int first, int c) {
+    int n = 0;
+    for (int b = thread_x() % 64; b < p.B; b += 64) {
+        const int q = b < 64 ? first : pages_at(p, b);
+        n += max((q + c - 1) / c, 1);
+    }
+    return wave_sum_i(n);
+}
+// Pages of a part, the same for every sequence: only the device knows the lengths, so every wave works it out for itself.  The
+// least (in steps of p.least, one step of the kernel a wave) for which all parts run at once, p.slots workgroups: a workgroup's
+// start and end cost as much as several pages.  Long sequences: about 1024 workgroups, of 64 pages at least, so that the CUs
+// finish together.  `first`: pages of sequence lane.
+__device__ __forceinline__ int part_pages(const AttendParams &p, int first, int64_t units, int most) {
+    constexpr int LONG = 64, ROUNDS = 1024;
+    int64_t work = 0;
+    for (int b = thread_x() % 64; b < p.B; b += 64) work += b < 64 ? first : pages_at(p, b);
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) work += __shfl_xor(work, o, 64);
+    work *= units;
+    int c = (int)min((work + p.slots - 1) / p.slots + p.least - 1, (int64_t)LONG) / p.least * p.least;
+    c = max(c, p.least);
+    for (int k = 0; k < 6 && c < LONG && p.B * units < p.slots; ++k) {
+        if (parts_in_all(p, first, c) * units <= p.slots) return c;
+        c = (c + c / 4 + p.least) / p.least * p.least;
+    }
+    return uni((int)min((int64_t)most, max((int64_t)LONG, (work + ROUNDS - 1) / ROUNDS)));
+}
+
 // KIND 1, 4: own rows by the few form with that many; 0: by the wide form.  NC: 16-row sets of the prefix's tiles (0: no prefix).
 // ALONE: every wave takes a sequence's own rows of one head by itself.
-template <typename TQ, typename TS, int D, int KIND, int NC, bool ALONE> __global__ __launch_bounds__(64 * waves(D)) void fpa_attend_kernel(AttendParams p) {
+// One row over e4m3 pages at D <= 64 keeps to 128 registers: four waves a SIMD (B4 H12 L65536: 84 us, 91 with three).
+template <typename TQ, typename TS, int D, int KIND> constexpr int waves_a_simd() {
+    return KIND == 1 && sizeof(TQ) == 2 && sizeof(TS) == 1 && D <= 64 ? 4 : waves(D) / 4;
+}
+template <typename TQ, typename TS, int D, int KIND, int NC, bool ALONE>
+__global__ __launch_bounds__(64 * waves(D), (waves_a_simd<TQ, TS, D, KIND>())) void fpa_attend_kernel(AttendParams p) {
     constexpr int NW = waves(D);
     __shared__ __align__(16) Shared<D, (NC ? NC : 1)> sh;
     __shared__ __align__(16) TQ weights[KIND ? NW : 1][KIND ? KIND * PG : 1];
     int64_t id = group_x();
-    const int H = p.c.H;
+    const int H = p.c.H, nrt = (p.N + CW - 1) / CW;  // tiles of a sequence's rows
+    const int lane = thread_x() % 64, units = H * nrt;
+    int first = 0;
+    if constexpr (!ALONE) {
+        if (p.nchunk > 1) {
+            first = pages_at(p, lane);
+            p.chunk = uni(part_pages(p, first, units, most_pages(D)));
+        }
+    }
     if constexpr (NC > 0) {
         constexpr int ROWS = tile_rows<NC>();
         const int tiles = (int)(((int64_t)p.B * p.N + ROWS - 1) / ROWS);
@@ -1197,24 +1265,46 @@ template <typename TQ, typename TS, int D, int KIND, int NC, bool ALONE> __globa
         }
         id -= npre;
     }
-    const int nrt = (p.N + CW - 1) / CW;  // tiles of a sequence's rows
     if constexpr (ALONE) {
         id = id * NW + uni(thread_x() / 64);
         if (id >= (int64_t)p.B * H * nrt) {
             if (p.npchunk > 0) own_done<TQ, D>(p, false, 0, 0, sh);  // the others' barriers
             return;
         }
+        // waves of a workgroup: one head, the same tiles
+        const int tile = (int)(id % nrt), h = (int)(id / nrt / p.B), b = (int)(id / nrt % p.B);
+        if constexpr (KIND > 0)
+            few_rows<TQ, TS, D, KIND, true>(p, b, h, 0, sh, weights);
+        else
+            wide_rows<TQ, TS, D, 1, false, true>(p, b, h, tile, 0, sh);
+    } else {
+        // item j = id / units of the sequences' parts in a row
+        int j = (int)(id / units), b = p.nchunk > 1 ? -1 : j, part = 0;
+        for (int b0 = 0; b0 < p.B && p.nchunk > 1; b0 += 64) {
+            const int q = b0 == 0 ? first : pages_at(p, b0 + lane);
+            int n = b0 + lane < p.B ? max((q + p.chunk - 1) / p.chunk, 1) : 0;
+            const int mine = n;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const int u = __shfl_up(n, o, 64);
+                if (lane >= o) n += u;
+            }
+            const uint64_t behind = __ballot(n > j);
+            if (behind) {
+                const int l = __builtin_ctzll(behind);
+                b = b0 + l;
+                part = uni(j - __shfl(n - mine, l, 64));
+                break;
+            }
+            j -= __builtin_amdgcn_readlane(n, 63);
+        }
+        if (b < 0) return;
+        const int h = (int)(id % units) / nrt, tile = (int)(id % units) % nrt;
+        if constexpr (KIND > 0)
+            few_rows<TQ, TS, D, KIND, false>(p, b, h, part, sh, weights);
+        else
+            wide_rows<TQ, TS, D, 1, false, false>(p, b, h, tile, part, sh);
     }
-    const int tile = (int)(id % nrt);
-    id /= nrt;
-    const int bh = (int)(id % ((int64_t)p.B * H)), part = (int)(id / ((int64_t)p.B * H));
-    const int b = ALONE ? bh % p.B : bh / H, h = ALONE ? bh / p.B : bh % H;  // waves of a workgroup: one head, the same tiles
-    bool lost = false;
-    if (!ALONE && part >= own_parts(p, seq_len(p, b, lost))) return;
-    if constexpr (KIND > 0)
-        few_rows<TQ, TS, D, KIND, ALONE>(p, b, h, part, sh, weights);
-    else
-        wide_rows<TQ, TS, D, 1, false, ALONE>(p, b, h, tile, part, sh);
 }
 
 // Row tiles of the prefix: 32 rows where there are more than 16 and their accumulators fit (fp16 to D = 128, fp32 to 64).
@@ -1251,7 +1341,7 @@ template <typename TQ, typename TS, int D, int KIND, int NC> void launch_attend_
             hipLaunchKernelGGL((fpa_attend_kernel<TQ, TS, D, KIND, NC, true>), dim3((uint32_t)(pre + (own + NW - 1) / NW)), dim3(64 * NW), 0, s, p);
             return;
         }
-    hipLaunchKernelGGL((fpa_attend_kernel<TQ, TS, D, KIND, NC, false>), dim3((uint32_t)(pre + own * p.nchunk)), dim3(64 * NW), 0, s, p);
+    hipLaunchKernelGGL((fpa_attend_kernel<TQ, TS, D, KIND, NC, false>), dim3((uint32_t)(pre + p.own_groups)), dim3(64 * NW), 0, s, p);
 }
 
 template <typename TQ, typename TS, int D> hipError_t launch_attend_d(const AttendParams &p, hipStream_t s) {

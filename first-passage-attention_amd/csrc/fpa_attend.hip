@@ -25,13 +25,7 @@ int attend_waves(int D) { return waves(D); }
 
 int attend_rows(int64_t rows, int D, int dtype) { return CW * prefix_sets(D, rows, dtype == ST_F32); }
 
-#ifndef PARTS_WG
-#define PARTS_WG 256
-#endif
-#ifndef ALONE_PAGES
-#define ALONE_PAGES 16
-#define ALONE_ITEMS 256
-#endif
+constexpr int CUS = 256;  // workgroups of the attention that run at once: one a CU, by their registers
 
 int attend_steps(int D, int dtype, int store, int64_t N, bool prefix, int sets) {
     const int kind = N > 4 ? 0 : N > 1 || prefix ? 4 : 1;
@@ -44,7 +38,7 @@ void attend_parts(int64_t items, int64_t pages, int D, int steps, int64_t taken,
     // As many parts as fill the CUs once, beside the `taken` workgroups that run with them: a workgroup's start and end cost as
     // much as several pages.  At most 64 pages, so that long sequences among short ones are spread in any case.
     const int least = waves(D) / steps > 1 ? waves(D) / steps : 1;  // one step a wave
-    const int64_t room = PARTS_WG - taken > PARTS_WG / 2 ? PARTS_WG - taken : PARTS_WG / 2;
+    const int64_t room = CUS - taken > CUS / 2 ? CUS - taken : CUS / 2;
     const int64_t want = items >= room ? 1 : room / items;
     int64_t c = ((pages + want - 1) / want + least - 1) / least * least;  // the same for every wave
     c = c > 64 ? 64 : c;
@@ -52,8 +46,26 @@ void attend_parts(int64_t items, int64_t pages, int D, int steps, int64_t taken,
     nchunk = (int)((pages + c - 1) / c);
 }
 
+void attend_own(int64_t B, int64_t units, int64_t pages, int D, int steps, int page_bytes, bool prefix, int &least, int &slots, int &nchunk, int64_t &groups) {
+    const auto larger = [](int64_t a, int64_t b) { return a > b ? a : b; };
+    least = waves(D) / steps > 1 ? waves(D) / steps : 1;
+    // A part is worth its start, its end and the join from about 32 KB of pages a wave on.
+    const int worth = waves(D) * (32 << 10) / page_bytes / least * least;
+    if (worth > least) least = worth;
+    slots = prefix ? CUS / 4 : CUS;
+    // What part_pages may come to: every part counted in the slots; or parts of 64 pages at least, about 1024 workgroups of them
+    // and one more for each item (unless a part at its largest still makes more).
+    const int64_t items = B * units, all = (pages + least - 1) / least, sixty = (pages + 63) / 64;
+    const int64_t most = items < slots ? larger(sixty, slots / units) : sixty;
+    nchunk = (int)(most < all ? most : all);
+    const int64_t largest = items * ((pages + most_pages(D) - 1) / most_pages(D));
+    const int64_t many = larger(1024, largest) + items, bound = items * sixty < many ? items * sixty : many;
+    groups = larger(bound, items < slots ? slots : 0);
+    if (groups > items * nchunk) groups = items * nchunk;
+}
+
 bool attend_alone(int64_t B, int64_t H, int64_t N, int64_t pages, int D, int dtype, bool prefix) {
-    return pages <= ALONE_PAGES && B * H >= ALONE_ITEMS && alone_built(N <= 4 ? 4 : 0, prefix ? prefix_sets(D, B * N, dtype == ST_F32) : 0);
+    return pages <= 16 && B * H >= CUS && alone_built(N <= 4 ? 4 : 0, prefix ? prefix_sets(D, B * N, dtype == ST_F32) : 0);
 }
 
 }  // namespace fpa

@@ -57,7 +57,9 @@ struct AttendParams {
     int32_t *counts;       // parts done of each (b, h), or (h, tile) with a prefix; 0 before and after every launch
     int B, N, P;
     int PL;                // positions of the shared prefix (0: none)
-    int chunk, nchunk;     // pages of a part, parts at most, of a sequence's own pages
+    int chunk, nchunk;     // pages of a part (set on the device), parts at most, of a sequence's own pages
+    int least, slots;      // a part's pages are a multiple of `least`; workgroups that run at once
+    int64_t own_groups;    // workgroups for the sequences' own pages
     int pchunk, npchunk;   // the same of the prefix (npchunk = 0: none)
     bool alone;            // a wave takes a sequence's own pages of a head by itself (nchunk = 1)
     float sc2;             // log2(e) / sqrt(D)
@@ -81,12 +83,14 @@ hipError_t launch_read(const MoveParams &p, int dtype, int store, hipStream_t s)
 hipError_t launch_attend(const AttendParams &p, int dtype, int store, int D, hipStream_t s);
 // Whether a wave takes all own pages of a sequence and head.
 bool attend_alone(int64_t B, int64_t H, int64_t N, int64_t pages, int D, int dtype, bool prefix);
-// Pages of a part and parts at most, for rows of at most `pages` pages; `items` counts the parts' other axes.
 int attend_rows(int64_t rows, int D, int dtype);  // rows of a tile of the prefix
 int attend_waves(int D);  // of a workgroup
 // Steps a page of the kernel, for a sequence's own N rows (sets = 0) or the prefix's tiles of 16 * sets rows.
 int attend_steps(int D, int dtype, int store, int64_t N, bool prefix, int sets);
+// Pages of the prefix's parts and their number.
 void attend_parts(int64_t items, int64_t pages, int D, int steps, int64_t taken, int &chunk, int &nchunk);
+// Sequences' own pages: least, slots, parts at most and workgroups (see AttendParams).
+void attend_own(int64_t B, int64_t units, int64_t pages, int D, int steps, int page_bytes, bool prefix, int &least, int &slots, int &nchunk, int64_t &groups);
 // Tokens of a span.
 int verify_span(int64_t B, int64_t V);
 hipError_t launch_verify(const VerifyParams &p, int dtype, hipStream_t s);

@@ -24,8 +24,21 @@ _HIP_NAMES = ("hip", "triton")
 
 
 def _refuse_grad(*tensors):
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-        raise ValueError("the serving operators have no gradient: call them under torch.no_grad()")
+    for t in tensors:
+        if t.requires_grad and torch.is_grad_enabled():
+            raise ValueError("the serving operators have no gradient: call them under torch.no_grad()")
+
+
+def _hip():
+    """The binding of the kernels; importing it loads libfpa.so and raises if it is missing."""
+    global _BINDING
+    if _BINDING is None:
+        from . import _serve
+        _BINDING = _serve
+    return _BINDING
+
+
+_BINDING = None
 
 
 def pick_impl(impl, t):
@@ -93,16 +106,21 @@ class PagedCache:
         self.dtype, self.device = k.dtype, k.device
         self._packed = None
 
-    def _check(self, B, table, dtype, **vectors):
-        if dtype not in (torch.float16, torch.float32):
+    def _check(self, B, table, dtype, start, name, counts=None):
+        if dtype is not self.dtype:
+            if dtype not in (torch.float16, torch.float32):
+                raise ValueError("the tensors must be fp16 or fp32")
+            if self.dtype is not torch.float8_e4m3fn:
+                raise ValueError(f"a cache of {self.dtype} takes and gives tensors of that type")
+        elif dtype is torch.float8_e4m3fn:
             raise ValueError("the tensors must be fp16 or fp32")
-        if self.dtype != STORES[2] and dtype != self.dtype:
-            raise ValueError(f"a cache of {self.dtype} takes and gives tensors of that type")
-        if table.dim() != 2 or table.shape[0] != B or table.shape[1] < 1 or table.dtype != torch.int32 or table.device != self.device:
+        dev = self.device
+        if table.dtype is not torch.int32 or table.dim() != 2 or table.shape[0] != B or table.shape[1] < 1 or table.device != dev:
             raise ValueError("table must be (B, P) int32 with P >= 1, on the cache's device")
-        for name, t in vectors.items():
-            if t is not None and (t.shape != (B,) or t.dtype != torch.int32 or t.device != self.device):
-                raise ValueError(f"{name} must be (B,) int32, on the cache's device")
+        if start.dtype is not torch.int32 or start.shape != (B,) or start.device != dev:
+            raise ValueError(f"{name} must be (B,) int32, on the cache's device")
+        if counts is not None and (counts.dtype is not torch.int32 or counts.shape != (B,) or counts.device != dev):
+            raise ValueError("counts must be (B,) int32, on the cache's device")
 
     def append(self, k, v, phi, psi, table, start, counts=None, impl=None):
         """Writes k, v (B, H, N, D), phi, psi (B, H, N) to positions start[b] + i, for i < counts[b] (all N without
@@ -115,15 +133,14 @@ class PagedCache:
             raise ValueError("k and v must hold at least one sequence and one position")
         if phi.shape != (B, H, N) or psi.shape != (B, H, N):
             raise ValueError("phi and psi must have shape (B, H, N)")
-        self._check(B, table, k.dtype, start=start, counts=counts)
-        for name, t in (("k", k), ("v", v), ("phi", phi), ("psi", psi)):
-            if t.device != self.device:
-                raise ValueError(f"{name} is on {t.device}, but the cache is on {self.device}")
+        self._check(B, table, k.dtype, start, "start", counts)
+        dev = self.device
+        if k.device != dev or v.device != dev or phi.device != dev or psi.device != dev:
+            raise ValueError(f"k, v, phi and psi must be on the cache's device, {dev}")
         _refuse_grad(k, v, phi, psi)
         if pick_impl(impl, self.k) == "reference":
             return dense.append(self, k, v, phi, psi, table, start, counts)
-        from ._serve import append  # loads libfpa.so; raises if it is missing
-        append(self, k, v, phi, psi, table, start, counts)
+        _hip().append(self, k, v, phi, psi, table, start, counts)
 
     def read(self, table, start, n, counts=None, dtype=None, impl=None):
         """k, v (B, H, n, D) and phi, psi (B, H, n) of positions start[b] + i; zero for i >= counts[b].  dtype: of k and v,
@@ -132,30 +149,31 @@ class PagedCache:
         dtype = dtype or (torch.float16 if self.dtype == STORES[2] else self.dtype)
         if n < 1 or B < 1:
             raise ValueError("at least one sequence and one position are read")
-        self._check(B, table, dtype, start=start, counts=counts)
+        self._check(B, table, dtype, start, "start", counts)
         if pick_impl(impl, self.k) == "reference":
             return dense.read(self, table, start, n, counts, dtype)
-        from ._serve import read
-        return read(self, table, start, n, counts, dtype)
+        return _hip().read(self, table, start, n, counts, dtype)
 
 
 def _check_attention(q, cache, beta, table, lengths):
     """Validation of both attention entry points; returns beta as (H,) float32."""
-    if q.dim() != 4 or q.shape[1] != cache.n_heads or q.shape[3] != cache.d_head or 0 in q.shape:
-        raise ValueError(f"q must be (B, {cache.n_heads}, N, {cache.d_head}) with B, N >= 1")
-    cache._check(q.shape[0], table, q.dtype, lengths=lengths)
+    shape = q.shape
+    H = cache.n_heads
+    if len(shape) != 4 or shape[1] != H or shape[3] != cache.d_head or shape[0] < 1 or shape[2] < 1:
+        raise ValueError(f"q must be (B, {H}, N, {cache.d_head}) with B, N >= 1")
+    cache._check(shape[0], table, q.dtype, lengths, "lengths")
     if not torch.is_tensor(beta):
         beta = torch.tensor(float(beta), device=q.device)
-    beta = beta.reshape(-1)
-    if beta.numel() == 1:
-        beta = beta.expand(cache.n_heads)
-    if beta.shape != (cache.n_heads,):
-        raise ValueError("beta must have shape (H,) or a single value")
-    for name, t in (("q", q), ("beta", beta)):
-        if t.device != cache.device:
-            raise ValueError(f"{name} is on {t.device}, but the cache is on {cache.device}")
+    if beta.shape != (H,):
+        beta = beta.reshape(-1)
+        if beta.numel() == 1:
+            beta = beta.expand(H)
+        if beta.shape != (H,):
+            raise ValueError("beta must have shape (H,) or a single value")
+    if q.device != cache.device or beta.device != cache.device:
+        raise ValueError(f"q and beta must be on the cache's device, {cache.device}")
     _refuse_grad(q, beta)
-    return beta.float()
+    return beta if beta.dtype is torch.float32 else beta.float()
 
 
 def cached_attention(q, cache, beta, table, lengths, impl=None):
@@ -169,8 +187,7 @@ def cached_attention(q, cache, beta, table, lengths, impl=None):
     beta = _check_attention(q, cache, beta, table, lengths)
     if pick_impl(impl, q) == "reference":
         return dense.attention(q, cache, beta, table, lengths)
-    from ._serve import attend
-    return attend(q, cache, beta, table, lengths, None, 0)
+    return _hip().attend(q, cache, beta, table, lengths, None, 0)
 
 
 def shared_prefix_attention(q, cache, beta, prefix, prefix_length, table, lengths, impl=None):
@@ -185,5 +202,4 @@ def shared_prefix_attention(q, cache, beta, prefix, prefix_length, table, length
         raise ValueError(f"prefix_length must be between 0 and the {PAGE * prefix.shape[0]} positions of its pages")
     if pick_impl(impl, q) == "reference":
         return dense.attention(q, cache, beta, table, lengths, prefix, prefix_length)
-    from ._serve import attend
-    return attend(q, cache, beta, table, lengths, prefix, prefix_length)
+    return _hip().attend(q, cache, beta, table, lengths, prefix, prefix_length)

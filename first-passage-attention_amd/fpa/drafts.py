@@ -2,7 +2,7 @@
 import torch
 
 from . import dense_serving as dense
-from .cache import _refuse_grad, pick_impl
+from .cache import _hip, _refuse_grad, pick_impl
 
 
 def verify_drafts(target, draft, tokens, accept_u, sample_u, impl=None):
@@ -33,11 +33,12 @@ def verify_drafts(target, draft, tokens, accept_u, sample_u, impl=None):
         raise ValueError("tokens must be int64")
     if accept_u.shape != (B, N) or sample_u.shape != (B,) or accept_u.dtype != torch.float32 or sample_u.dtype != torch.float32:
         raise ValueError("accept_u must be (B, N) and sample_u (B,), float32")
-    for name, t in (("draft", draft), ("tokens", tokens), ("accept_u", accept_u), ("sample_u", sample_u)):
-        if t is not None and t.device != target.device:
-            raise ValueError(f"{name} is on {t.device}, but target is on {target.device}")
-    _refuse_grad(target, *([] if draft is None else [draft]))
+    dev = target.device
+    if tokens.device != dev or accept_u.device != dev or sample_u.device != dev or (draft is not None and draft.device != dev):
+        raise ValueError(f"draft, tokens, accept_u and sample_u must be on target's device, {dev}")
+    _refuse_grad(target)
+    if draft is not None:
+        _refuse_grad(draft)
     if pick_impl(impl, target) == "reference":
         return dense.verify(target, draft, tokens, accept_u, sample_u)
-    from ._serve import verify
-    return verify(target, draft, tokens, accept_u, sample_u)
+    return _hip().verify(target, draft, tokens, accept_u, sample_u)
