@@ -560,7 +560,7 @@ int fpa_attend(const FpaAttendArgs *a, void *stream) {
 int64_t fpa_verify_workspace_bytes(int64_t B, int64_t V) {
     if (B < 1 || V < 1) return 0;
     const int64_t span = verify_span(B, V), spans = (V + span - 1) / span;
-    return (B * spans * 16 + B * 4 + 255) / 256 * 256;
+    return B * spans * 4 * 16;  // four waves a span, two doubles each
 }
 
 int fpa_verify(const FpaVerifyArgs *a, void *stream) {
@@ -574,11 +574,12 @@ int fpa_verify(const FpaVerifyArgs *a, void *stream) {
         return fail(FPA_ERR_INVALID, "target, tokens, accept_u, sample_u, accepted and out must be non-NULL");
     if (a->workspace == nullptr || (reinterpret_cast<uintptr_t>(a->workspace) & 255) != 0)
         return fail(FPA_ERR_INVALID, "workspace must be non-NULL and 256-byte aligned");
+    if (!a->counts || (reinterpret_cast<uintptr_t>(a->counts) & 3) != 0) return fail(FPA_ERR_INVALID, "counts must be non-NULL");
     VerifyParams p = {};
     p.span = verify_span(a->B, a->V);
     p.spans = (int)((a->V + p.span - 1) / p.span);
     p.sums = static_cast<double *>(a->workspace);
-    p.none = reinterpret_cast<int32_t *>(p.sums + a->B * p.spans * 2);
+    p.counts = a->counts;
     p.target = a->target; p.stb = a->st[0]; p.stn = a->st[1];
     p.draft = a->N > 0 ? a->draft : nullptr; p.sdb = a->sd[0]; p.sdn = a->sd[1];
     p.tokens = a->tokens; p.sxb = a->sx;

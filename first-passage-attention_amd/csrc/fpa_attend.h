@@ -313,6 +313,9 @@ __device__ __forceinline__ f32x2 get2(const float *p) {
 
 __device__ __forceinline__ float exp_or_0(float m, float ref) { return fexp2(m - (ref == ninf() ? 0.f : ref)); }
 
+// Long sequences are cut into about LONG_GROUPS parts in all, of LONG_PART pages at least.
+constexpr int LONG_PART = 48, LONG_GROUPS = 1024;
+
 // Rows of a prefix tile.
 template <int NC> constexpr int tile_rows() { return CW * NC; }
 
@@ -566,7 +569,7 @@ __device__ __forceinline__ void few_rows(const AttendParams &p, int b, int h, in
     // Everything that names a page first, then what those name: two trips to memory before the first scores.
     const int pages = page_numbers(p, table, ws, T0 < T1 ? we : ws, lane, missing);
     const bool far = pf > (ALONE ? we : ps) + PG;  // more whole pages behind than one load of the wave covers
-    const int near_end = far && !ALONE ? min(pe, pf) : min(pf, we + PG);
+    const int near_end = min(far && !ALONE ? min(pe, pf) : pf, we + PG);
     const int behind_page = page_numbers(p, table, we, T0 < T1 ? near_end : 0, lane, missing);
     const int part_page = page_numbers(p, table, max(we, pf), T0 < T1 ? npg : 0, lane, missing);  // at most two
     float mine = T0 < T1 && we + lane < near_end ? p.c.phi_min[(int64_t)behind_page * H + h] : pinf();
@@ -606,11 +609,11 @@ __device__ __forceinline__ void few_rows(const AttendParams &p, int b, int h, in
     }  // rows past N repeat the last: never written
     const float beta2 = p.beta[h] * LOG2E;
 
-    // min of phi from the wave's pages on: whole pages, those beyond the next 64 by all waves together, then the at most
+    // min of phi from the wave's pages on: whole pages, those behind the part by all waves together where there are many, then the at most
     // two pages that some rows see in part
     float carry[NR];
     {
-        if (ALONE && far) mine = fminf(mine, lane_min(p, table, h, we + PG + lane, pf, 64, missing));
+        if (far && T0 < T1) mine = fminf(mine, lane_min(p, table, h, we + PG + lane, ALONE ? pf : min(pe, pf), 64, missing));
         mine = wave_min(mine);
         if (!ALONE && far) {
             const float m = wave_min(lane_min(p, table, h, pe + tid, pf, 64 * NW, missing));
@@ -884,7 +887,7 @@ __device__ __forceinline__ void wide_rows(const AttendParams &p, int b0, int h, 
     const int cut = T1 % HT * KT;                     // keys of the last that are the wave's, 0: all
     const int pages = page_numbers(p, table, ws, T0 < T1 ? we : ws, lane, missing);
     const bool far = pf > (ALONE ? we : ps) + PG;
-    const int near_end = far && !ALONE ? min(pe, pf) : min(pf, we + PG);
+    const int near_end = min(far && !ALONE ? min(pe, pf) : pf, we + PG);
     const int behind_page = page_numbers(p, table, we, T0 < T1 ? near_end : 0, lane, missing);
     const int part_page = page_numbers(p, table, max(we, pf), T0 < T1 ? npg : 0, lane, missing);
     float mine = T0 < T1 && we + lane < near_end ? p.c.phi_min[(int64_t)behind_page * H + h] : pinf();
@@ -959,7 +962,7 @@ __device__ __forceinline__ void wide_rows(const AttendParams &p, int b0, int h, 
     }
     const float beta2 = p.beta[h] * LOG2E;
     {
-        if (ALONE && far) mine = fminf(mine, lane_min(p, table, h, we + PG + lane, pf, 64, missing));
+        if (far && T0 < T1) mine = fminf(mine, lane_min(p, table, h, we + PG + lane, ALONE ? pf : min(pe, pf), 64, missing));
         mine = wave_min(mine);
         if (!ALONE && far) {
             const float mb = wave_min(lane_min(p, table, h, pe + tid, pf, 64 * NW, missing));
@@ -1211,23 +1214,29 @@ __device__ __forceinline__ int parts_in_all(const AttendParams &p, int first, in
     return wave_sum_i(n);
 }
 // Pages of a part, the same for every sequence: only the device knows the lengths, so every wave works it out for itself.  The
-// least (in steps of p.least, one step of the kernel a wave) for which all parts run at once, p.slots workgroups: a workgroup's
-// start and end cost as much as several pages.  Long sequences: about 1024 workgroups, of 64 pages at least, so that the CUs
-// finish together.  `first`: pages of sequence lane.
+// least (a multiple of p.least) for which all parts run at once, p.slots workgroups: a workgroup's start and end cost as much as
+// several pages.  Where that takes LONG_PART pages or more: parts of LONG_PART pages or of so many that there are LONG_GROUPS
+// of them, so that the CUs finish together.  `first`: pages of sequence lane.  Never more than p.nchunk parts of a
+// sequence, which is what the workspace holds.
 __device__ __forceinline__ int part_pages(const AttendParams &p, int first, int64_t units, int most) {
-    constexpr int LONG = 64, ROUNDS = 1024;
     int64_t work = 0;
     for (int b = thread_x() % 64; b < p.B; b += 64) work += b < 64 ? first : pages_at(p, b);
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) work += __shfl_xor(work, o, 64);
     work *= units;
-    int c = (int)min((work + p.slots - 1) / p.slots + p.least - 1, (int64_t)LONG) / p.least * p.least;
-    c = max(c, p.least);
-    for (int k = 0; k < 6 && c < LONG && p.B * units < p.slots; ++k) {
+    const int floor = max(p.least, (p.P + p.nchunk - 1) / p.nchunk);
+    int c = max((int)min((work + p.slots - 1) / p.slots + p.least - 1, (int64_t)LONG_PART) / p.least * p.least, floor);
+    for (int k = 0; k < 6 && c < LONG_PART && p.B * units < p.slots; ++k) {
         if (parts_in_all(p, first, c) * units <= p.slots) return c;
         c = (c + c / 4 + p.least) / p.least * p.least;
     }
-    return uni((int)min((int64_t)most, max((int64_t)LONG, (work + ROUNDS - 1) / ROUNDS)));
+    c = (int)min((int64_t)most, max((int64_t)LONG_PART, (work + LONG_GROUPS - 1) / LONG_GROUPS));
+    for (int k = 0; k < 6 && c < most; ++k) {  // nor a few more than the slots
+        const int64_t n = parts_in_all(p, first, c) * units;
+        if (n <= p.slots || (n >= 2 * p.slots && n <= LONG_GROUPS)) break;
+        c = min(c + (c + 15) / 16, most);
+    }
+    return max(c, floor);
 }
 
 // KIND 1, 4: own rows by the few form with that many; 0: by the wide form.  NC: 16-row sets of the prefix's tiles (0: no prefix).

@@ -48,20 +48,20 @@ void attend_parts(int64_t items, int64_t pages, int D, int steps, int64_t taken,
 
 void attend_own(int64_t B, int64_t units, int64_t pages, int D, int steps, int page_bytes, bool prefix, int &least, int &slots, int &nchunk, int64_t &groups) {
     const auto larger = [](int64_t a, int64_t b) { return a > b ? a : b; };
+    const auto smaller = [](int64_t a, int64_t b) { return a < b ? a : b; };
     least = waves(D) / steps > 1 ? waves(D) / steps : 1;
     // A part is worth its start, its end and the join from about 32 KB of pages a wave on.
     const int worth = waves(D) * (32 << 10) / page_bytes / least * least;
     if (worth > least) least = worth;
     slots = prefix ? CUS / 4 : CUS;
-    // What part_pages may come to: every part counted in the slots; or parts of 64 pages at least, about 1024 workgroups of them
-    // and one more for each item (unless a part at its largest still makes more).
-    const int64_t items = B * units, all = (pages + least - 1) / least, sixty = (pages + 63) / 64;
-    const int64_t most = items < slots ? larger(sixty, slots / units) : sixty;
-    nchunk = (int)(most < all ? most : all);
-    const int64_t largest = items * ((pages + most_pages(D) - 1) / most_pages(D));
-    const int64_t many = larger(1024, largest) + items, bound = items * sixty < many ? items * sixty : many;
-    groups = larger(bound, items < slots ? slots : 0);
-    if (groups > items * nchunk) groups = items * nchunk;
+    // What part_pages may come to.  Fewer items than slots: either all parts of all sequences fit the slots, so that one sequence
+    // has at most slots / units of them; or, as with more items, a part has LONG_PART pages at least (and `least` in any case).
+    const int64_t items = B * units, all = (pages + least - 1) / least, cut = (pages + LONG_PART - 1) / LONG_PART;
+    nchunk = (int)smaller(all, items < slots ? larger(cut, larger(slots / units, 1)) : cut);
+    // Workgroups: in the second case parts of work / LONG_GROUPS pages (or the most that a part may have), rounded up a sequence.
+    const int64_t fullest = items * ((pages + most_pages(D) - 1) / most_pages(D));
+    groups = smaller(items * cut, larger(LONG_GROUPS, fullest) + items);
+    groups = smaller(items < slots ? larger(groups, slots) : groups, items * nchunk);
 }
 
 bool attend_alone(int64_t B, int64_t H, int64_t N, int64_t pages, int D, int dtype, bool prefix) {

@@ -86,19 +86,10 @@ template <typename TX> struct Piece {
     }
 };
 
-template <typename TS> __device__ __forceinline__ float value(TS x, int e) {
-    if constexpr (sizeof(TS) == 1) {
-        const float v = __builtin_amdgcn_cvt_f32_fp8(x.code, 0);
-        return v * pow2(e);
-    } else {
-        return (float)x;
-    }
-}
-
 template <typename TX, typename TS, int D>
 __global__ __launch_bounds__(256) void fpa_append_kernel(MoveParams p) {
     constexpr int N16 = Piece<TX>::N, LPR = D / N16, RPP = 256 / LPR;  // lanes of a row, rows of a pass
-    constexpr int LP = D + 16 / sizeof(TS);                              // pitch of the V tile in LDS
+    constexpr int LP = D + (sizeof(TS) == 1 ? 4 : 16 / (int)sizeof(TS));   // pitch of the V tile in LDS
     __shared__ __align__(16) TS tile[PG * LP];
     const int tid = thread_x(), h = group_y(), b = group_z();
     const int64_t start = p.start[b];
@@ -154,20 +145,52 @@ __global__ __launch_bounds__(256) void fpa_append_kernel(MoveParams p) {
         if (tid == 0) p.c.phi_min[ph] = x;
     }
     __syncthreads();
-    // V^T: four positions of one feature per thread and step.
-    for (int e = tid; e < D * PG / 4; e += 256) {
-        const int d = e / (PG / 4), s = e % (PG / 4) * 4;
+    // V^T: the positions of one feature, in pieces of 16 bytes where the page is written whole.
+    constexpr int PC = 16 / sizeof(TS);
+    if (lo == 0 && hi == PG) {
+        for (int e = tid; e < D * PG / PC; e += 256) {
+            const int d = e / (PG / PC), r = e % (PG / PC) * PC;
+            uint32_t w[4];
+            TS *x = reinterpret_cast<TS *>(w);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (s + i >= lo && s + i < hi) cv[d * PG + s + i] = tile[(s + i) * LP + d];
+            for (int i = 0; i < PC; ++i) x[i] = tile[(r + i) * LP + d];
+            *reinterpret_cast<u32x4 *>(cv + d * PG + r) = u32x4{w[0], w[1], w[2], w[3]};
+        }
+    } else {
+        const int n = hi - lo;
+        for (int e = tid; e < D * n; e += 256) {
+            const int d = e / n, r = lo + e % n;
+            cv[d * PG + r] = tile[r * LP + d];
+        }
+    }
+}
+
+// N consecutive cache values as float, times the row's power of two.
+template <typename TS, int N> __device__ __forceinline__ void values(float (&x)[N], const TS *p, float scale) {
+    if constexpr (sizeof(TS) == 1) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+            const int w = *reinterpret_cast<const int *>(p + i);
+            const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8(w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
+            x[i] = a[0] * scale;
+            x[i + 1] = a[1] * scale;
+            x[i + 2] = b[0] * scale;
+            x[i + 3] = b[1] * scale;
+        }
+    } else {
+        Piece<TS> q;
+        q.load(p);
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = q.x[i];
     }
 }
 
 template <typename TX, typename TS, int D>
 __global__ __launch_bounds__(256) void fpa_read_kernel(MoveParams p) {
-    constexpr int LP = PG + 16 / sizeof(TS);
-    __shared__ __align__(16) TS tile[D * LP];
-    __shared__ int8_t ve[PG];
+    constexpr int PC = 16 / sizeof(TS);   // positions of a piece of V^T
+    constexpr int LP = D + (sizeof(TS) == 1 ? 4 : 16 / (int)sizeof(TS));  // V rows by position in LDS
+    constexpr int N16 = Piece<TX>::N, LPR = D / N16;
+    __shared__ __align__(16) TS tile[PG * LP];
     const int tid = thread_x(), h = group_y(), b = group_z();
     int64_t start = p.start[b];
     int64_t n = p.counts ? p.counts[b] : p.N;
@@ -187,24 +210,38 @@ __global__ __launch_bounds__(256) void fpa_read_kernel(MoveParams p) {
     const TS *ck = static_cast<const TS *>(p.c.k) + ph * PG * D;
     const TS *cv = static_cast<const TS *>(p.c.v) + ph * PG * D;
     const int64_t row0 = ((int64_t)b * p.c.H + h) * p.N + i0;
-    for (int e = tid; e < D * PG && there; e += 256) tile[e / PG * LP + e % PG] = cv[e];
-    if (sizeof(TS) == 1 && tid < PG && there) ve[tid] = p.c.v_exp[ph * PG + tid];
+    if (there) {
+        if (hi - lo > PG / 4) {  // the page's V, turned
+            for (int e = tid; e < D * PG / PC; e += 256) {
+                const int d = e / (PG / PC), r = e % (PG / PC) * PC;
+                const u32x4 w = *reinterpret_cast<const u32x4 *>(cv + d * PG + r);
+                const TS *x = reinterpret_cast<const TS *>(&w);
+#pragma unroll
+                for (int i = 0; i < PC; ++i) tile[(r + i) * LP + d] = x[i];
+            }
+        } else {  // a few positions
+            const int m = hi - lo;
+            for (int e = tid; e < D * m; e += 256) tile[(lo + e % m) * LP + e / m] = cv[e / m * PG + lo + e % m];
+        }
+    }
     __syncthreads();
     const float nan = __uint_as_float(0x7fc00000u);
-    for (int e = lo * D + tid; e < hi * D; e += 256) {
-        const int r = e / D, d = e % D;
-        float kx = 0.f, vx = 0.f;
-        if (i0 + r < n) {
-            kx = vx = nan;
-            if (there) {
-                int ke = 0, vv = 0;
-                if constexpr (sizeof(TS) == 1) { ke = p.c.k_exp[ph * PG + r]; vv = ve[r]; }
-                kx = value(ck[e], ke);
-                vx = value(tile[d * LP + r], vv);
+    for (int e = lo * LPR + tid; e < hi * LPR; e += 256) {
+        const int r = e / LPR, col = e % LPR * N16;
+        Piece<TX> k, v;
+#pragma unroll
+        for (int i = 0; i < N16; ++i) k.x[i] = v.x[i] = i0 + r < n ? nan : 0.f;
+        if (there && i0 + r < n) {
+            float ks = 1.f, vs = 1.f;
+            if constexpr (sizeof(TS) == 1) {
+                ks = pow2(p.c.k_exp[ph * PG + r]);
+                vs = pow2(p.c.v_exp[ph * PG + r]);
             }
+            values<TS, N16>(k.x, ck + r * D + col, ks);
+            values<TS, N16>(v.x, tile + r * LP + col, vs);
         }
-        static_cast<TX *>(p.ko)[(row0 + r) * D + d] = (TX)kx;
-        static_cast<TX *>(p.vo)[(row0 + r) * D + d] = (TX)vx;
+        k.store(static_cast<TX *>(p.ko) + (row0 + r) * D + col);
+        v.store(static_cast<TX *>(p.vo) + (row0 + r) * D + col);
     }
     if (tid >= lo && tid < hi) {
         const bool in = i0 + tid < n;

@@ -72,8 +72,8 @@ struct VerifyParams {
     const float *accept_u; int64_t sub;
     const float *sample_u;
     int64_t *accepted, *out;
-    double *sums;  // (B, spans, 2): of each span's tokens
-    int32_t *none; // (B,): no token at the rejected position
+    double *sums;     // (B, 4 spans, 2): of each quarter of a span
+    int32_t *counts;  // (B,): spans done; 0 before and after every launch
     int B, N, V;
     int span, spans;
 };

@@ -67,53 +67,6 @@ template <typename T> __device__ int first_rejected(const VerifyParams &a, const
     return a.N;
 }
 
-// Sums of each span of a sequence's row: sums[b][span] = (rest, target).  Every workgroup finds the rejected
-// position for itself; the first of a sequence keeps it for the second kernel.
-template <typename T> __global__ __launch_bounds__(VT) void fpa_verify_sum_kernel(VerifyParams a) {
-    __shared__ double part[2 * VW];
-    __shared__ int first, none;
-    const int b = group_y(), span = group_x(), lane = thread_x() % 64, wave = thread_x() / 64;
-    const T *p = static_cast<const T *>(a.target) + (int64_t)b * a.stb;
-    const T *q = a.draft ? static_cast<const T *>(a.draft) + (int64_t)b * a.sdb : nullptr;
-    const int64_t *x = a.tokens + (int64_t)b * a.sxb;
-    if (wave == 0) {
-        bool no;
-        const int n = first_rejected(a, p, q, x, a.accept_u + (int64_t)b * a.sub, no);
-        if (lane == 0) {
-            first = n;
-            none = no;
-            if (span == 0) {
-                a.accepted[b] = n;
-                a.none[b] = no;
-            }
-        }
-    }
-    __syncthreads();
-    const int n = first;
-    const bool no = none;
-    const Row<T> row = {p + (int64_t)n * a.stn, q && !no ? q + (int64_t)n * a.sdn : nullptr, no ? -1 : x[n]};
-    const int v0 = span * a.span, v1 = min(v0 + a.span, a.V);
-    double rest = 0.0, target = 0.0;
-#pragma unroll 4
-    for (int v = v0 + thread_x(); v < v1; v += VT) {
-        rest += row.rest(v);
-        target += row.target(v);
-    }
-    rest = wave_sum(rest);
-    target = wave_sum(target);
-    if (lane == 0) {
-        part[2 * wave] = rest;
-        part[2 * wave + 1] = target;
-    }
-    __syncthreads();
-    if (thread_x() < 2) {
-        double s = part[thread_x()];
-#pragma unroll
-        for (int w = 1; w < VW; ++w) s += part[2 * w + thread_x()];
-        a.sums[2 * ((int64_t)b * a.spans + span) + thread_x()] = s;
-    }
-}
-
 // Inclusive sums of one value per thread in thread order; total gets the sum of all.
 __device__ __forceinline__ double block_sums(double x, double *part, double &total) {
     const int lane = thread_x() % 64, wave = thread_x() / 64;
@@ -152,25 +105,70 @@ __device__ __forceinline__ int block_pick(bool over, bool some, int *pick) {
     return pick[0] < VT ? pick[0] : pick[1];
 }
 
-// Draws the token: the span that the target falls into, then the token in the span; sums that round below the target
-// fall to the last one with any weight.
-template <typename T> __global__ __launch_bounds__(VT) void fpa_verify_draw_kernel(VerifyParams a) {
+// Values that another workgroup of this launch reads: agent-scope accesses, past the caches that the XCDs do not share.
+__device__ __forceinline__ void put(double *p, double x) {
+    __hip_atomic_store(reinterpret_cast<uint64_t *>(p), __builtin_bit_cast(uint64_t, x), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ double get(const double *p) {
+    return __builtin_bit_cast(double, __hip_atomic_load(reinterpret_cast<const uint64_t *>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+}
+
+// One workgroup a span of a sequence's row; each finds the rejected position for itself, and each wave sums a quarter of the
+// span: sums[b][VW * span + wave] = (rest, target).  The workgroup that finishes a sequence's last span draws the token:
+// the quarter that the target falls into, then the token in it; sums that round below the target fall to the last token with
+// any weight.
+template <typename T> __global__ __launch_bounds__(VT) void fpa_verify_kernel(VerifyParams a) {
     __shared__ double part[VW], at;
-    __shared__ int pick[2], found;
-    const int b = group_x(), tid = thread_x();
-    const int64_t *x = a.tokens + (int64_t)b * a.sxb;
-    const int n = (int)a.accepted[b];
-    const bool no = a.none[b] != 0;
+    __shared__ int first, none, last, pick[2], found;
+    const int b = group_y(), span = group_x(), tid = thread_x(), lane = tid % 64, wave = tid / 64;
+    const T *p = static_cast<const T *>(a.target) + (int64_t)b * a.stb;
     const T *q = a.draft ? static_cast<const T *>(a.draft) + (int64_t)b * a.sdb : nullptr;
-    const Row<T> row = {static_cast<const T *>(a.target) + (int64_t)b * a.stb + (int64_t)n * a.stn,
-                        q && !no ? q + (int64_t)n * a.sdn : nullptr, no ? -1 : x[n]};
-    const double *sums = a.sums + 2 * (int64_t)b * a.spans;
-    // a thread's spans: EACH neighbouring ones
-    const int each = (a.spans + VT - 1) / VT, s0 = min(tid * each, a.spans), s1 = min(s0 + each, a.spans);
+    const int64_t *x = a.tokens + (int64_t)b * a.sxb;
+    if (wave == 0) {
+        bool no;
+        const int n = first_rejected(a, p, q, x, a.accept_u + (int64_t)b * a.sub, no);
+        if (lane == 0) {
+            first = n;
+            none = no;
+        }
+    }
+    __syncthreads();
+    const int n = first;
+    const bool no = none;
+    const Row<T> row = {p + (int64_t)n * a.stn, q && !no ? q + (int64_t)n * a.sdn : nullptr, no ? -1 : x[n]};
+    const int quarter = a.span / VW, subs = a.spans * VW;
+    double *sums = a.sums + 2 * (int64_t)b * subs;
+    {
+        const int v0 = (int)min((int64_t)span * a.span + wave * quarter, (int64_t)a.V), v1 = min(v0 + quarter, a.V);
+        double rest = 0.0, target = 0.0;
+#pragma unroll 4
+        for (int v = v0 + lane; v < v1; v += 64) {
+            rest += row.rest(v);
+            target += row.target(v);
+        }
+        rest = wave_sum(rest);
+        target = wave_sum(target);
+        if (lane == 0) {
+            put(sums + 2 * (span * VW + wave), rest);
+            put(sums + 2 * (span * VW + wave) + 1, target);
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        }
+    }
+    __syncthreads();
+    if (tid == 0) {
+        int32_t *count = a.counts + b;
+        last = __hip_atomic_fetch_add(count, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1 == a.spans;
+        if (last) __hip_atomic_store(count, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // for the next launch
+    }
+    __syncthreads();
+    if (!last) return;
+
+    // a thread's quarters: `each` neighbouring ones
+    const int each = (subs + VT - 1) / VT, s0 = min(tid * each, subs), s1 = min(s0 + each, subs);
     double rest = 0.0, target = 0.0;
     for (int s = s0; s < s1; ++s) {
-        rest += sums[2 * s];
-        target += sums[2 * s + 1];
+        rest += get(sums + 2 * s);
+        target += get(sums + 2 * s + 1);
     }
     double total;
     double upto = block_sums(rest, part, total);
@@ -181,24 +179,23 @@ template <typename T> __global__ __launch_bounds__(VT) void fpa_verify_draw_kern
         const double goal = (double)a.sample_u[b] * total, mine = use_rest ? rest : target;
         int who = block_pick(mine > 0.0 && upto > goal, mine > 0.0, pick);
         if (tid == who) {
-            double run = upto - mine;
-            if (s0 == 0) run = 0.0;
-            int s = s0, last = s0;
-            double last_run = run;
-            for (; s < s1; ++s) {
-                const double w = sums[2 * s + !use_rest];
+            double run = s0 == 0 ? 0.0 : upto - mine, last_run = run;
+            int in = s0;
+            for (int s = s0; s < s1; ++s) {
+                const double w = get(sums + 2 * s + !use_rest);
                 if (w > 0.0) {
-                    last = s;
+                    in = s;
                     last_run = run;
                     if (run + w > goal) break;
                 }
                 run += w;
             }
-            found = last;
+            found = in;
             at = last_run;
         }
         __syncthreads();
-        const int v0 = found * a.span, v1 = min(v0 + a.span, a.V);
+        const int64_t f = (int64_t)(found / VW) * a.span + found % VW * quarter;
+        const int v0 = (int)f, v1 = (int)min(f + quarter, (int64_t)a.V);
         const int per = (v1 - v0 + VT - 1) / VT, t0 = min(v0 + tid * per, v1), t1 = min(t0 + per, v1);
         double w = 0.0;
         for (int v = t0; v < t1; ++v) w += use_rest ? row.rest(v) : row.target(v);
@@ -208,28 +205,29 @@ template <typename T> __global__ __launch_bounds__(VT) void fpa_verify_draw_kern
         who = block_pick(w > 0.0 && end > goal, w > 0.0, pick);
         if (tid == who) {
             double run = end - w;
-            int last = -1;
+            int in = -1;
             for (int v = t0; v < t1; ++v) {
                 const double y = use_rest ? row.rest(v) : row.target(v);
                 run += y;
                 if (y > 0.0) {
-                    last = v;
+                    in = v;
                     if (run > goal) break;
                 }
             }
-            found = last;
+            found = in;
         }
         __syncthreads();
         token = found;
     }
     for (int i = tid; i <= a.N; i += VT) a.out[(int64_t)b * (a.N + 1) + i] = i < n ? x[i] : i == n ? token : -1;
+    if (tid == 0) a.accepted[b] = n;
 }
 
 }  // namespace
 
 int verify_span(int64_t B, int64_t V) {
     // Spans of a multiple of 1024 tokens, about 2048 workgroups in all (eight on a CU, 4096 tokens each at the most
-    // common sizes).  B64 V128003 fp32: see the table beside fpa_verify_sum_kernel.
+    // common sizes).
     int64_t per = (B * V + 2047) / 2048;
     per = per < V ? per : V;
     per = (per + 1023) / 1024 * 1024;
@@ -237,17 +235,10 @@ int verify_span(int64_t B, int64_t V) {
 }
 
 hipError_t launch_verify(const VerifyParams &p, int dtype, hipStream_t s) {
-    if (dtype == ST_F16) {
-        hipLaunchKernelGGL((fpa_verify_sum_kernel<f16>), dim3(p.spans, p.B), dim3(VT), 0, s, p);
-        hipError_t e = hipGetLastError();
-        if (e != hipSuccess) return e;
-        hipLaunchKernelGGL((fpa_verify_draw_kernel<f16>), dim3(p.B), dim3(VT), 0, s, p);
-    } else {
-        hipLaunchKernelGGL((fpa_verify_sum_kernel<float>), dim3(p.spans, p.B), dim3(VT), 0, s, p);
-        hipError_t e = hipGetLastError();
-        if (e != hipSuccess) return e;
-        hipLaunchKernelGGL((fpa_verify_draw_kernel<float>), dim3(p.B), dim3(VT), 0, s, p);
-    }
+    if (dtype == ST_F16)
+        hipLaunchKernelGGL((fpa_verify_kernel<f16>), dim3(p.spans, p.B), dim3(VT), 0, s, p);
+    else
+        hipLaunchKernelGGL((fpa_verify_kernel<float>), dim3(p.spans, p.B), dim3(VT), 0, s, p);
     return hipGetLastError();
 }
 

@@ -98,7 +98,7 @@ class FpaVerifyArgs(ctypes.Structure):
     _fields_ = [("B", _i64), ("N", _i64), ("V", _i64), ("dtype", ctypes.c_int32),
                 ("target", _vp), ("st", _S2), ("draft", _vp), ("sd", _S2), ("tokens", _vp), ("sx", _i64),
                 ("accept_u", _vp), ("su", _i64), ("sample_u", _vp), ("accepted", _vp), ("out", _vp),
-                ("workspace", _vp)]
+                ("workspace", _vp), ("counts", _vp)]
 
 
 # Their byte images, as above; a cache's own part is packed once and kept with it.
@@ -107,7 +107,7 @@ _CACHE = f"={PAGES_PACK.size}sqqqi4x"
 APPEND_PACK = struct.Struct(_CACHE + "q4q" * 2 + "q3q" * 2 + "qqqq")
 READ_PACK = struct.Struct(_CACHE + "qqqq" + "qqqq")
 ATTEND_PACK = struct.Struct(_CACHE + "q4q" * 2 + "q" + "qqq" + "qq" + "qq")
-VERIFY_PACK = struct.Struct("=qqqi4x" + "q2q" * 2 + "qq" * 2 + "qqqq")
+VERIFY_PACK = struct.Struct("=qqqi4x" + "q2q" * 2 + "qq" * 2 + "qqqqq")
 assert [x.size for x in (PAGES_PACK, APPEND_PACK, READ_PACK, ATTEND_PACK, VERIFY_PACK)] == [
     ctypes.sizeof(x) for x in (FpaPages, FpaAppendArgs, FpaReadArgs, FpaAttendArgs, FpaVerifyArgs)]
 

@@ -84,10 +84,12 @@ def attend(q, c, beta, table, lengths, prefix, prefix_length):
     os = (N * H * D, D, H * D, 1)  # (B, N, H, D) in memory
     with device_guard(dev):
         o = torch.empty_strided((B, H, N, D), os, dtype=dtype, device=dev)
+        # held until the launch: a captured graph's pool would give the memory of one that is gone to the next
+        ws, counts = workspace(dev, nws) if nws else None, counters(dev, ncounts)
         a = _lib.FpaAttendArgs.from_buffer_copy(_lib.ATTEND_PACK.pack(
             _pages(c), B, N, P, _CODES[dtype], q.data_ptr(), *qs, o.data_ptr(), *os, beta.data_ptr(),
             table.data_ptr(), table.stride(0), lengths.data_ptr(), _ptr(prefix), prefix_length,
-            workspace(dev, nws).data_ptr() if nws else 0, counters(dev, ncounts).data_ptr()))
+            _ptr(ws), counts.data_ptr()))
         _lib.check(_lib.lib().fpa_attend(a, _lib.stream_of(dev)))
     return o
 
@@ -105,9 +107,10 @@ def verify(target, draft, tokens, accept_u, sample_u):
     with device_guard(dev):
         both = torch.empty(B * (N + 2), dtype=torch.int64, device=dev)  # both results in one allocation
         at = both.data_ptr()
+        ws, counts = workspace(dev, _verify_ws_bytes(B, V)), counters(dev, B)  # held until the launch, as above
         a = _lib.FpaVerifyArgs.from_buffer_copy(_lib.VERIFY_PACK.pack(
             B, N, V, _CODES[target.dtype], target.data_ptr(), ts[0], ts[1], _ptr(draft), ds[0], ds[1],
             tokens.data_ptr(), tokens.stride(0), accept_u.data_ptr(), accept_u.stride(0), sample_u.data_ptr(), at, at + 8 * B,
-            workspace(dev, _verify_ws_bytes(B, V)).data_ptr()))
+            ws.data_ptr(), counts.data_ptr()))
         _lib.check(_lib.lib().fpa_verify(a, _lib.stream_of(dev)))
     return both[:B], both[B:].view(B, N + 1)

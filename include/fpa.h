@@ -291,6 +291,7 @@ typedef struct {
     int64_t *accepted;
     int64_t *out;                          /* contiguous */
     void *workspace;                       /* fpa_verify_workspace_bytes(), 256-byte aligned */
+    int32_t *counts;                       /* B ints, as FpaAttendArgs.counts */
 } FpaVerifyArgs;
 int64_t fpa_verify_workspace_bytes(int64_t B, int64_t V);
 int fpa_verify(const FpaVerifyArgs *args, void *stream);

@@ -159,6 +159,17 @@ def test_long_sequences_in_parts(store, q, D, N):
     assert torch.equal(a, cached_attention(x[:, :, :N], cache, beta, table, L))
 
 
+@pytest.mark.parametrize("store,q,D", [("e4m3", "f16", 16), ("e4m3", "f32", 16), ("f16", "f16", 16), ("f32", "f32", 128)])
+def test_very_long_sequences(store, q, D):
+    """Small pages, of which a part holds more than of others (D = 16), and parts of 48 pages; one long sequence, and one among
+    short ones in a table that is far too wide."""
+    cache, table, L, _, x, beta = filled(3, 2, D, [16500, 40, 9000], store, q, D, width=400, device=DEV)
+    for b in (slice(0, 1), slice(0, 3)):
+        for N in (1, 2):
+            o = cached_attention(x[b, :, :N], cache, beta, table[b], L[b])
+            held(o, *want64(x[b, :, :N], cache, beta, table[b], L[b]), 4 * TOL[q])  # sums over 16500 positions
+
+
 @pytest.mark.parametrize("store,q", MOVES)
 @pytest.mark.parametrize("P", [1, 64, 100, 777])
 def test_prefix(store, q, P):
