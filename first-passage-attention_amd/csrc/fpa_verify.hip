@@ -141,7 +141,7 @@ template <typename T> __global__ __launch_bounds__(VT) void fpa_verify_kernel(Ve
     {
         const int v0 = (int)min((int64_t)span * a.span + wave * quarter, (int64_t)a.V), v1 = min(v0 + quarter, a.V);
         double rest = 0.0, target = 0.0;
-#pragma unroll 4
+#pragma unroll 8
         for (int v = v0 + lane; v < v1; v += 64) {
             rest += row.rest(v);
             target += row.target(v);

@@ -143,6 +143,24 @@ class Field(nn.Module):
         w = delta.cumsum(dim=-1)
         return w + g, w + h, F.softplus(self.beta_raw)
 
+    def _terms(self, x):
+        """delta, g, h (B, H, T) of x in fp32."""
+        B, T, _ = x.shape
+        with torch.autocast(device_type=x.device.type, enabled=False):
+            lin = F.linear(x.float(), self.proj.weight.float(), self.proj.bias.float())
+        return lin.view(B, T, 3, self.n_heads).permute(2, 0, 3, 1)
+
+    def last_w(self, x, phi, last):
+        """W (B, H) at position last (B,) of a prompt whose phi forward(x) gave: what `extend` goes on from."""
+        _, g, _ = self._terms(x[torch.arange(x.shape[0], device=x.device), last].unsqueeze(1))
+        return phi.gather(2, last.view(-1, 1, 1).expand(-1, phi.shape[1], 1)).squeeze(2) - g.squeeze(2)
+
+    def extend(self, x, w):
+        """phi, psi (B, H, N), beta and W (B, H, N) of N new positions x (B, N, C) behind those that ended at W = w (B, H)."""
+        delta, g, h = self._terms(x)
+        w = w.unsqueeze(2) + delta.cumsum(dim=-1)
+        return w + g, w + h, F.softplus(self.beta_raw), w
+
 
 class FirstPassageAttention(nn.Module):
     """Multi-head causal FPA without positional encoding: x (B, T, d_model) -> (B, T, d_model)
@@ -166,3 +184,39 @@ class FirstPassageAttention(nn.Module):
         phi, psi, beta = self.field(x)
         o = _attention_packed(qkv, phi, psi, beta, self.tau, self.impl, self.block)  # (B, T, H, D)
         return self.out(o.reshape(B, T, -1))
+
+    # Serving, without gradients: a prompt runs as in training and leaves its positions in a cache; a few new positions
+    # attend to what the cache holds.
+
+    def new_cache(self, pages, x, store=None):
+        """A cache of this layer on x's device, of type `store` or that of the projection of x (autocast's, if on)."""
+        if store is None:
+            dev = x.device.type
+            store = torch.get_autocast_dtype(dev) if torch.is_autocast_enabled(dev) else self.qkv.weight.dtype
+        return PagedCache(pages, self.h, self.d, store, device=x.device)
+
+    @torch.no_grad()
+    def prompt(self, x, cache, table, counts):
+        """forward(x) of prompts x (B, T, d_model), of which sequence b has counts[b] positions (int32), appended to `cache`.
+        Returns (output, W of the last positions)."""
+        B, T, _ = x.shape
+        qkv = self.qkv(x).view(B, T, 3, self.h, self.d)
+        phi, psi, beta = self.field(x)
+        o = _attention_packed(qkv, phi, psi, beta, self.tau, self.impl, self.block)
+        _, k, v = qkv.permute(2, 0, 3, 1, 4)
+        cache.append(k, v, phi.float(), psi.float(), table, torch.zeros_like(counts), counts, impl=self.impl)
+        return self.out(o.reshape(B, T, -1)), self.field.last_w(x, phi.float(), counts.long() - 1)
+
+    @torch.no_grad()
+    def extend(self, x, cache, table, lengths, w, prefix=None):
+        """N new positions x (B, N, d_model) behind `lengths` cached ones that ended at W = w; prefix: None or (pages, length) of
+        a shared one.  Appends them; returns (output, W (B, H, N))."""
+        B, N, _ = x.shape
+        q, k, v = self.qkv(x).view(B, N, 3, self.h, self.d).permute(2, 0, 3, 1, 4)
+        phi, psi, beta, w = self.field.extend(x, w)
+        cache.append(k, v, phi, psi, table, lengths, impl=self.impl)
+        if prefix is None:
+            o = cached_attention(q, cache, beta, table, lengths + N, impl=self.impl)
+        else:
+            o = shared_prefix_attention(q, cache, beta, *prefix, table, lengths + N, impl=self.impl)
+        return self.out(o.transpose(1, 2).reshape(B, N, -1)), w
