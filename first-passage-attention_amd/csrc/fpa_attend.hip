@@ -64,8 +64,13 @@ void attend_own(int64_t B, int64_t units, int64_t pages, int D, int steps, int p
     groups = smaller(items < slots ? larger(groups, slots) : groups, items * nchunk);
 }
 
+// A wave alone takes its pages one after the other, but needs no fold and no more workgroups than an eighth of the sequences.
+// Beside a prefix's parts, which fill the CUs, that is what keeps all in one round (B32 H12 D64 P16381: 42 -> 26 us); by
+// themselves short sequences have to be so many that their waves fill the CUs (B33 H12 L742, 400 of them: 33 us alone, 17 in
+// workgroups of their own).
 bool attend_alone(int64_t B, int64_t H, int64_t N, int64_t pages, int D, int dtype, bool prefix) {
-    return pages <= 16 && B * H >= CUS && alone_built(N <= 4 ? 4 : 0, prefix ? prefix_sets(D, B * N, dtype == ST_F32) : 0);
+    const bool many = prefix ? pages <= 16 && B * H >= CUS : (pages <= 8 && B * H >= 3 * CUS) || (pages <= 4 && B * H >= 2 * CUS);
+    return many && alone_built(N <= 4 ? 4 : 0, prefix ? prefix_sets(D, B * N, dtype == ST_F32) : 0);
 }
 
 }  // namespace fpa

@@ -159,6 +159,26 @@ def test_long_sequences_in_parts(store, q, D, N):
     assert torch.equal(a, cached_attention(x[:, :, :N], cache, beta, table, L))
 
 
+@pytest.mark.parametrize("store,q", [("f16", "f16"), ("e4m3", "f32")])
+@pytest.mark.parametrize("prefix", [0, 70])
+def test_many_short_sequences(store, q, prefix):
+    """So many that a wave takes each by itself; with odd sizes, so that the last workgroup is not full."""
+    g = torch.Generator().manual_seed(11)
+    B = 61
+    lengths = [0, 1, 256, 64] + torch.randint(0, 257, (B - 4,), generator=g).tolist()
+    cache, table, L, pre, x, beta = filled(B, 9, 32, lengths, store, q, 1, prefix=prefix, device=DEV)
+    for N in (1, 3):
+        if prefix:
+            o = shared_prefix_attention(x[:, :, :N], cache, beta, pre, prefix, table, L)
+        else:
+            o = cached_attention(x[:, :, :N], cache, beta, table, L)
+        held(o, *want64(x[:, :, :N], cache, beta, table, L, pre, prefix), TOL[q])
+        t = table.clone()
+        t[2, 3] = -1
+        bad = shared_prefix_attention(x[:, :, :N], cache, beta, pre, prefix, t, L) if prefix else cached_attention(x[:, :, :N], cache, beta, t, L)
+        assert bad[2].isnan().all() and torch.equal(bad[:2], o[:2]) and torch.equal(bad[3:], o[3:])
+
+
 @pytest.mark.parametrize("store,q,D", [("e4m3", "f16", 16), ("e4m3", "f32", 16), ("f16", "f16", 16), ("f32", "f32", 128)])
 def test_very_long_sequences(store, q, D):
     """Small pages, of which a part holds more than of others (D = 16), and parts of 48 pages; one long sequence, and one among
