@@ -1241,12 +1241,8 @@ __device__ __forceinline__ int part_pages(const AttendParams &p, int first, int6
 
 // KIND 1, 4: own rows by the few form with that many; 0: by the wide form.  NC: 16-row sets of the prefix's tiles (0: no prefix).
 // ALONE: every wave takes a sequence's own rows of one head by itself.
-// One row over e4m3 pages at D <= 64 keeps to 128 registers: four waves a SIMD (B4 H12 L65536: 84 us, 91 with three).
-template <typename TQ, typename TS, int D, int KIND> constexpr int waves_a_simd() {
-    return KIND == 1 && sizeof(TQ) == 2 && sizeof(TS) == 1 && D <= 64 ? 4 : waves(D) / 4;
-}
 template <typename TQ, typename TS, int D, int KIND, int NC, bool ALONE>
-__global__ __launch_bounds__(64 * waves(D), (waves_a_simd<TQ, TS, D, KIND>())) void fpa_attend_kernel(AttendParams p) {
+__global__ __launch_bounds__(64 * waves(D)) void fpa_attend_kernel(AttendParams p) {
     constexpr int NW = waves(D);
     __shared__ __align__(16) Shared<D, (NC ? NC : 1)> sh;
     __shared__ __align__(16) TQ weights[KIND ? NW : 1][KIND ? KIND * PG : 1];
