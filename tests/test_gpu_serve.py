@@ -210,6 +210,38 @@ def test_prefix_head_sizes_and_many_rows(D):
         held(o, *want64(x[:, :, :N], cache, beta, table, L, pre, 200), TOL["f16"])
 
 
+@pytest.mark.parametrize("store,q", MOVES)
+@pytest.mark.parametrize("D", [16, 32, 64, 128, 256])
+def test_prefix_of_every_kernel(store, q, D):
+    """Every type and head size with tiles of 16 and of 32 rows, own rows in both forms, and own pages in several parts."""
+    for B, lengths in ((3, [70, 2, 1800]), (9, [33, 64, 65, 1, 300, 0, 16, 1700, 90])):
+        cache, table, L, pre, x, beta = filled(B, 2, D, lengths, store, q, D, prefix=200, device=DEV)
+        for N in (1, 5):
+            o = shared_prefix_attention(x[:, :, :N], cache, beta, pre, 200, table, L)
+            held(o, *want64(x[:, :, :N], cache, beta, table, L, pre, 200), TOL[q])
+
+
+@pytest.mark.parametrize("N", [20, 43])
+def test_prefix_with_more_rows_than_a_tile(N):
+    cache, table, L, pre, x, beta = filled(3, 2, 64, [130, 1700, 25], "f16", "f16", N, prefix=130, device=DEV)
+    x = torch.cat([x, x.flip(2), x * 0.5], 2)[:, :, :N]
+    for b in (slice(0, 1), slice(0, 3)):
+        o = shared_prefix_attention(x[b], cache, beta, pre, 130, table[b], L[b])
+        held(o, *want64(x[b], cache, beta, table[b], L[b], pre, 130), TOL["f16"])
+
+
+@pytest.mark.parametrize("store,q", MOVES)
+@pytest.mark.parametrize("D", [16, 64, 128, 256])
+def test_waves_alone_of_every_kernel(store, q, D):
+    g = torch.Generator().manual_seed(D)
+    lengths = torch.randint(0, 257, (48,), generator=g).tolist()
+    cache, table, L, pre, x, beta = filled(48, 16, D, lengths, store, q, 1, prefix=64, device=DEV)
+    for N in (1, 2):
+        held(cached_attention(x[:, :, :N], cache, beta, table, L), *want64(x[:, :, :N], cache, beta, table, L), TOL[q])
+    o = shared_prefix_attention(x[:, :, :2], cache, beta, pre, 64, table, L)
+    held(o, *want64(x[:, :, :2], cache, beta, table, L, pre, 64), TOL[q])
+
+
 def test_prefix_equals_its_copy_in_every_table():
     """The prefix in front of each sequence's own pages (a whole number of pages) through cached_attention."""
     P = 192
