@@ -53,6 +53,9 @@ def pick_impl(impl, t):
     return "hip"
 
 
+_FIXED = frozenset(("k", "v", "phi", "psi", "phi_min", "k_exp", "v_exp", "pages", "n_heads", "d_head", "dtype", "device"))
+
+
 class PagedCache:
     """Pages of 64 positions for the heads of one attention layer.
 
@@ -104,7 +107,15 @@ class PagedCache:
         self.k, self.v, self.phi, self.psi, self.phi_min, self.k_exp, self.v_exp = k, v, phi, psi, phi_min, k_exp, v_exp
         self.pages, self.n_heads, self.d_head = n, H, D
         self.dtype, self.device = k.dtype, k.device
-        self._packed = None
+        self._packed = None  # the kernels' argument block, with the buffers' addresses
+
+    def __setattr__(self, name, value):
+        if name in _FIXED and name in self.__dict__:
+            raise AttributeError(f"a cache keeps its {name}: PagedCache.from_buffers makes one of other buffers")
+        super().__setattr__(name, value)
+
+    def __getstate__(self):  # of copies, whose buffers may be others
+        return {**self.__dict__, "_packed": None}
 
     def _check(self, B, table, dtype, start, name, counts=None):
         if dtype is not self.dtype:

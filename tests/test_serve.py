@@ -1,5 +1,6 @@
 """The serving operators on the CPU: impl="reference" against the float64 oracle, and every refusal (also of the C ABI,
 which validates before any launch)."""
+import copy
 import ctypes
 import os
 import shutil
@@ -187,6 +188,17 @@ def test_refusals_of_the_cache():
             pytest.fail(f"call {i} was not refused")
     with pytest.raises(RuntimeError):
         c.append(k, v, phi, psi, table, start, impl="hip")
+
+
+def test_buffers_stay_and_copies_have_their_own():
+    """The argument block of a cache is kept with it: its buffers cannot be exchanged, and a copy starts without the block."""
+    c = fpa.PagedCache(2, 1, 16)
+    with pytest.raises(AttributeError, match="from_buffers"):
+        c.k = torch.zeros_like(c.k)
+    c._packed = b"addresses of the buffers"
+    d = copy.deepcopy(c)
+    assert d._packed is None and d.k.data_ptr() != c.k.data_ptr() and torch.equal(d.phi_min, c.phi_min)
+    d.name = "further attributes are the caller's"
 
 
 def test_refusals_of_the_attention():
