@@ -151,9 +151,12 @@ class Field(nn.Module):
         return lin.view(B, T, 3, self.n_heads).permute(2, 0, 3, 1)
 
     def last_w(self, x, phi, last):
-        """W (B, H) at position last (B,) of a prompt whose phi forward(x) gave: what `extend` goes on from."""
-        _, g, _ = self._terms(x[torch.arange(x.shape[0], device=x.device), last].unsqueeze(1))
-        return phi.gather(2, last.view(-1, 1, 1).expand(-1, phi.shape[1], 1)).squeeze(2) - g.squeeze(2)
+        """W (B, H) at position last (B,) of a prompt whose phi forward(x) gave (0 for -1, before the first): what `extend`
+        goes on from."""
+        at = last.clamp(0, x.shape[1] - 1)
+        _, g, _ = self._terms(x[torch.arange(x.shape[0], device=x.device), at].unsqueeze(1))
+        w = phi.gather(2, at.view(-1, 1, 1).expand(-1, phi.shape[1], 1)).squeeze(2) - g.squeeze(2)
+        return torch.where((last < 0).unsqueeze(1), 0., w)
 
     def extend(self, x, w):
         """phi, psi (B, H, N), beta and W (B, H, N) of N new positions x (B, N, C) behind those that ended at W = w (B, H)."""

@@ -80,15 +80,23 @@ class FPADecoder(nn.Module):
     @torch.no_grad()
     def start(self, tokens, room, counts=None, samples=None, store=None):
         """Reads prompts (B, T), sequence b of counts[b] tokens (all T without counts), and returns (logits (B, vocab) behind the
-        last of each, DecodeState with room for `room` more positions a sequence).  samples: continue the one prompt that often;
-        its positions are then kept once.  store: the caches' type, torch.float8_e4m3fn for 8 bits (None: the activations')."""
+        last of each, DecodeState with room for `room` more positions a sequence; beyond that logits are NaN).  samples: continue
+        the one prompt that often; its positions are then kept once, and counts is None.  store: the caches' type,
+        torch.float8_e4m3fn for 8 bits (None: the activations')."""
         B, T = tokens.shape
         dev = tokens.device
-        if samples is not None and B != 1:
-            raise ValueError("samples are taken of one prompt")
-        counts = torch.full((B,), T, dtype=torch.int32, device=dev) if counts is None else counts.to(torch.int32)
+        if B < 1 or T < 1 or room < 0:
+            raise ValueError("start needs a prompt of at least one token and room >= 0")
+        if samples is not None and (B != 1 or samples < 1 or counts is not None):
+            raise ValueError("samples, one or more, are taken of one whole prompt")
+        if counts is None:
+            counts = torch.full((B,), T, dtype=torch.int32, device=dev)
+        else:
+            counts = counts.to(torch.int32)
+            if counts.shape != (B,) or bool(((counts < 1) | (counts > T)).any()):
+                raise ValueError("counts must be (B,), each between 1 and T")
         first = -(-(T if samples is not None else T + room) // PAGE)
-        own = -(-room // PAGE) if samples is not None else 0
+        own = max(-(-room // PAGE), 1) if samples is not None else 0
         table = torch.arange(B * first + (samples or 0) * own, dtype=torch.int32, device=dev)
         prompts, own_table = table[:B * first].view(B, first), table[B * first:].view(-1, own) if samples is not None else None
         x = self.emb(tokens)
@@ -129,7 +137,8 @@ def _sample(probs, u):
 @torch.no_grad()
 def generate(model, tokens, steps, counts=None, samples=None, draft=None, drafts=4, temperature=1.0, generator=None, store=None):
     """tokens (B, steps) int64 sampled behind the prompts `tokens` (see FPADecoder.start).  draft: a smaller model that proposes
-    `drafts` tokens at a time, of which `model` accepts what keeps its own distribution (verify_drafts)."""
+    `drafts` tokens at a time, of which `model` accepts what keeps its own distribution (verify_drafts).  Logits that are no
+    distribution (NaN) give -1, after which the sequence goes on as if behind token 0."""
     if steps < 1 or not temperature > 0 or (draft is not None and drafts < 1):
         raise ValueError("generate needs steps >= 1, temperature > 0 and drafts >= 1")
     dev = tokens.device
@@ -146,7 +155,7 @@ def generate(model, tokens, steps, counts=None, samples=None, draft=None, drafts
     if draft is None:
         out = [last]
         for _ in range(steps - 1):
-            out.append(_sample(probs(model.extend(state, out[-1])[:, 0]), uniform(B)))
+            out.append(_sample(probs(model.extend(state, out[-1].clamp(min=0))[:, 0]), uniform(B)))
         return torch.cat(out, 1)
     _, guess = draft.start(tokens, room, counts, samples, store)
     out = torch.full((B, steps + drafts + 1), -1, dtype=torch.int64, device=dev)
@@ -157,14 +166,14 @@ def generate(model, tokens, steps, counts=None, samples=None, draft=None, drafts
         base, w = guess.lengths, guess.w
         tried, q, ws = [last], [], []
         for i in range(drafts + 1):  # the last of them only enters the draft model's cache
-            p = probs(draft.extend(guess, tried[-1], keep=False)[:, 0])
+            p = probs(draft.extend(guess, tried[-1].clamp(min=0), keep=False)[:, 0])
             ws.append([x[..., 0] for x in guess._new])
             guess.keep(torch.ones_like(guess.lengths))
             if i < drafts:
                 q.append(p)
                 tried.append(_sample(p, uniform(B)))
         x = torch.cat(tried, 1)
-        p = probs(model.extend(state, x, keep=False))
+        p = probs(model.extend(state, x.clamp(min=0), keep=False))
         n, next_tokens = verify_drafts(p, torch.stack(q, 1), x[:, 1:].contiguous(), uniform(B, drafts), uniform(B))
         kept = torch.where(done < steps, n + 1, 0)  # sequences that are done stay where they are
         state.keep(kept.to(torch.int32))

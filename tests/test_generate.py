@@ -128,3 +128,51 @@ def test_half_precision_decoding_at_the_layers_size():
             got = [logits.unsqueeze(1)] + [m.extend(state, tokens[:, i:i + 1]) for i in range(300, 310)]
         got = torch.cat(got, 1).float()
         assert ((got - want[:, 299:]).norm() / want[:, 299:].norm()).item() <= tol
+
+
+def test_samples_are_of_one_whole_prompt():
+    m = model("cpu")
+    tokens = torch.zeros(1, 7, dtype=torch.int64)
+    with pytest.raises(ValueError, match="whole prompt"):
+        m.start(tokens, 4, counts=torch.tensor([3]), samples=2)
+    with pytest.raises(ValueError, match="samples"):
+        m.start(tokens, 4, samples=0)
+    with pytest.raises(ValueError, match="prompt"):
+        m.start(tokens[:, :0], 4)
+    with pytest.raises(ValueError, match="room"):
+        m.start(tokens, -1)
+    logits, state = m.start(tokens, 0, samples=2)  # no room: a table of one page all the same
+    assert logits.shape[0] == 2 and state.table.shape == (2, 1)
+
+
+@pytest.mark.parametrize("count", [0, 8, -1])
+def test_counts_outside_the_prompt_are_refused(count):
+    m = model("cpu")
+    with pytest.raises(ValueError, match="counts"):
+        m.start(torch.zeros(2, 7, dtype=torch.int64), 4, counts=torch.tensor([3, count]))
+
+
+def test_an_empty_prompt_of_a_layer_ends_at_zero():
+    """W starts at zero before a sequence's first position: extending a prompt of no positions is beginning a sequence."""
+    a = model("cpu").blocks[0].attn
+    x = torch.randn(2, 5, 64, generator=torch.Generator().manual_seed(3))
+    cache = a.new_cache(2, x)
+    table, counts = torch.tensor([[0], [1]], dtype=torch.int32), torch.tensor([0, 5], dtype=torch.int32)
+    _, w = a.prompt(x, cache, table, counts)
+    assert torch.equal(w[0], torch.zeros_like(w[0]))
+    y, _ = a.extend(x, cache, table, torch.zeros_like(counts), torch.zeros_like(w))
+    with torch.no_grad():
+        assert (y - a(x)).abs().max() <= TOL
+
+
+@pytest.mark.parametrize("drafted", [False, True])
+def test_logits_without_a_distribution_give_no_token(drafted):
+    """-1 in the answer, as verify_drafts gives it; it is never looked up as a token."""
+    m = model("cpu")
+    with torch.no_grad():
+        m.head.weight.fill_(float("nan"))
+    out = generate(m, torch.zeros(2, 5, dtype=torch.int64), 4, draft=model("cpu", 1, layers=1) if drafted else None, drafts=2)
+    assert torch.equal(out, torch.full((2, 4), -1))
+    if drafted:  # and drafts without one are none: the model's own tokens
+        out = generate(model("cpu"), torch.zeros(2, 5, dtype=torch.int64), 4, draft=m, drafts=2)
+        assert (out >= 0).all()
