@@ -313,8 +313,9 @@ __device__ __forceinline__ f32x2 get2(const float *p) {
 
 __device__ __forceinline__ float exp_or_0(float m, float ref) { return fexp2(m - (ref == ninf() ? 0.f : ref)); }
 
-// Long sequences are cut into about LONG_GROUPS parts in all, of LONG_PART pages at least.
-constexpr int LONG_PART = 48, LONG_GROUPS = 1024;
+// Workgroups of one round, one a CU; sequences that do not fit one round by parts of fewer than SHORT_PART pages are cut into parts
+// of LONG_PART pages at least, for up to ROUNDS of them.
+constexpr int CUS = 256, SHORT_PART = 48, LONG_PART = 24, ROUNDS = 4, LONG_GROUPS = ROUNDS * CUS;
 
 // Rows of a prefix tile.
 template <int NC> constexpr int tile_rows() { return CW * NC; }
@@ -1195,10 +1196,15 @@ __device__ __forceinline__ void wide_rows(const AttendParams &p, int b0, int h, 
     }
 }
 
+template <int CTRL, int ROWS> __device__ __forceinline__ int dpp_or_0(int x) { return __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, false); }
 __device__ __forceinline__ int wave_sum_i(int x) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) x += __shfl_xor(x, o, 64);
-    return x;
+    x += dpp_or_0<0x111, 0xf>(x);
+    x += dpp_or_0<0x112, 0xf>(x);
+    x += dpp_or_0<0x114, 0xf>(x);
+    x += dpp_or_0<0x118, 0xf>(x);
+    x += dpp_or_0<0x142, 0xa>(x);
+    x += dpp_or_0<0x143, 0xc>(x);
+    return __builtin_amdgcn_readlane(x, 63);
 }
 __device__ __forceinline__ int pages_at(const AttendParams &p, int b) {
     bool over = false;
@@ -1213,28 +1219,39 @@ __device__ __forceinline__ int parts_in_all(const AttendParams &p, int first, in
     }
     return wave_sum_i(n);
 }
-// Pages of a part, the same for every sequence: only the device knows the lengths, so every wave works it out for itself.  The
-// least (a multiple of p.least) for which all parts run at once, p.slots workgroups: a workgroup's start and end cost as much as
-// several pages.  Where that takes LONG_PART pages or more: parts of LONG_PART pages or of so many that there are LONG_GROUPS
-// of them, so that the CUs finish together.  `first`: pages of sequence lane.  Never more than p.nchunk parts of a
-// sequence, which is what the workspace holds.
+// Pages of a part, the same for every sequence: only the device knows the lengths, so every wave works it out for itself.
+// Never more than p.nchunk parts of a sequence, which is what the workspace holds.  `first`: pages of sequence lane.
+//   One part, if no sequence has more than two times p.least: the second step costs less than the join (B4 H12 D64 L1500 e4m3:
+//   9.9 us, 13.7 in two parts).
+//   Else the least multiple of p.least for which all parts run at once, p.slots workgroups (B16 H12 D64 L2048 fp16: 22.7 us; 43.8 where
+//   that was given up for 24 pages or more, 35 with two workgroups a CU).
+//   Where that takes SHORT_PART pages or more: parts for one workgroup a CU if they come out even (at most an eighth above the
+//   CU's share of the pages), else for two, else for four (B4 H12 D64 L65536 e4m3: 84.5, 86.9, 88.9 us; B16 H12, ragged to 20000:
+//   80, 65.0, 65.5).
 __device__ __forceinline__ int part_pages(const AttendParams &p, int first, int64_t units, int most) {
     int64_t work = 0;
-    for (int b = thread_x() % 64; b < p.B; b += 64) work += b < 64 ? first : pages_at(p, b);
+    int longest = 0;
+    for (int b = thread_x() % 64; b < p.B; b += 64) {
+        const int q = b < 64 ? first : pages_at(p, b);
+        work += q;
+        longest = max(longest, q);
+    }
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) work += __shfl_xor(work, o, 64);
     work *= units;
     const int floor = max(p.least, (p.P + p.nchunk - 1) / p.nchunk);
-    int c = max((int)min((work + p.slots - 1) / p.slots + p.least - 1, (int64_t)LONG_PART) / p.least * p.least, floor);
-    for (int k = 0; k < 6 && c < LONG_PART && p.B * units < p.slots; ++k) {
+    if (p.npchunk == 0 && !__any(longest > 2 * p.least)) return max(2 * p.least, floor);
+    int c = max((int)min((work + p.slots - 1) / p.slots + p.least - 1, (int64_t)SHORT_PART) / p.least * p.least, floor);
+    for (int k = 0; k < 6 && c < SHORT_PART && p.B * units < p.slots; ++k) {
         if (parts_in_all(p, first, c) * units <= p.slots) return c;
         c = (c + c / 4 + p.least) / p.least * p.least;
     }
-    c = (int)min((int64_t)most, max((int64_t)LONG_PART, (work + LONG_GROUPS - 1) / LONG_GROUPS));
-    for (int k = 0; k < 6 && c < most; ++k) {  // nor a few more than the slots
-        const int64_t n = parts_in_all(p, first, c) * units;
-        if (n <= p.slots || (n >= 2 * p.slots && n <= LONG_GROUPS)) break;
-        c = min(c + (c + 15) / 16, most);
+    for (int r = 1; r <= ROUNDS; r *= 2) {
+        c = (int)min((int64_t)most, max((int64_t)max(LONG_PART, floor), (work + r * CUS - 1) / (r * CUS)));
+        for (int k = 0; k < 4 && c < most; ++k) {
+            if (parts_in_all(p, first, c) * units <= r * CUS) return c;
+            if (k < 3) c = min(c + (c + 23) / 24, most);
+        }
     }
     return max(c, floor);
 }

@@ -25,8 +25,6 @@ int attend_waves(int D) { return waves(D); }
 
 int attend_rows(int64_t rows, int D, int dtype) { return CW * prefix_sets(D, rows, dtype == ST_F32); }
 
-constexpr int CUS = 256;  // workgroups of the attention that run at once: one a CU, by their registers
-
 int attend_steps(int D, int dtype, int store, int64_t N, bool prefix, int sets) {
     const int kind = N > 4 ? 0 : N > 1 || prefix ? 4 : 1;
     if (store == ST_F16) return steps_of<f16, f16>(D, kind, sets);
@@ -50,14 +48,18 @@ void attend_own(int64_t B, int64_t units, int64_t pages, int D, int steps, int p
     const auto larger = [](int64_t a, int64_t b) { return a > b ? a : b; };
     const auto smaller = [](int64_t a, int64_t b) { return a < b ? a : b; };
     least = waves(D) / steps > 1 ? waves(D) / steps : 1;
-    // A part is worth its start, its end and the join from about 32 KB of pages a wave on.
-    const int worth = waves(D) * (32 << 10) / page_bytes / least * least;
+    // A part is worth its start, its end and its share of the join from about 16 KB of pages a wave on (B2 H12 D64 L4000: e4m3
+    // 14.1 us, fp16 16.2; from 32 KB on 15.8 and 18.7).
+    const int worth = waves(D) * (16 << 10) / page_bytes / least * least;
     if (worth > least) least = worth;
     slots = prefix ? CUS / 4 : CUS;
     // What part_pages may come to.  Fewer items than slots: either all parts of all sequences fit the slots, so that one sequence
     // has at most slots / units of them; or, as with more items, a part has LONG_PART pages at least (and `least` in any case).
     const int64_t items = B * units, all = (pages + least - 1) / least, cut = (pages + LONG_PART - 1) / LONG_PART;
-    nchunk = (int)smaller(all, items < slots ? larger(cut, larger(slots / units, 1)) : cut);
+    if (!prefix && pages <= 2 * least)
+        nchunk = 1;
+    else
+        nchunk = (int)smaller(all, items < slots ? larger(cut, larger(slots / units, 1)) : cut);
     // Workgroups: in the second case parts of work / LONG_GROUPS pages (or the most that a part may have), rounded up a sequence.
     const int64_t fullest = items * ((pages + most_pages(D) - 1) / most_pages(D));
     groups = smaller(items * cut, larger(LONG_GROUPS, fullest) + items);
