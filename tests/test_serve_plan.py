@@ -37,12 +37,12 @@ def device(lens, units, pages, least, slots, nchunk, most, prefix):
     if not prefix and max(lens) <= 2 * least:
         return max(2 * least, floor)
     c = max(min(-(-work // slots) + least - 1, SHORT_PART) // least * least, floor)
-    for _ in range(6):
+    for _ in range(10):
         if not (c < SHORT_PART and B * units < slots):
             break
         if count(c) <= slots:
             return c
-        c = (c + c // 4 + least) // least * least
+        c = (c + c // 8 + least) // least * least
     for r in (1, 2, 4):
         c = min(most, max(LONG_PART, floor, -(-work // (r * CUS))))
         for k in range(4):
